@@ -87,6 +87,17 @@ void kv_store(torch::Tensor qkv, int64_t k_off, int64_t v_off, torch::Tensor slo
               torch::Tensor k_pages, torch::Tensor v_pages);
 void kv_gather(torch::Tensor qkv, int64_t k_off, int64_t v_off, torch::Tensor slots,
                torch::Tensor k_pages, torch::Tensor v_pages);
+void kv_store_fp8(torch::Tensor qkv, int64_t k_off, int64_t v_off, torch::Tensor slots,
+                  torch::Tensor k_pages, torch::Tensor v_pages, c10::optional<torch::Tensor> k_scales,
+                  c10::optional<torch::Tensor> v_scales);
+void kv_gather_fp8(torch::Tensor qkv, int64_t k_off, int64_t v_off, torch::Tensor slots,
+                   torch::Tensor k_pages, torch::Tensor v_pages, c10::optional<torch::Tensor> k_scales,
+                   c10::optional<torch::Tensor> v_scales);
+void paged_attention(torch::Tensor q, torch::Tensor k_pages, torch::Tensor v_pages,
+                     c10::optional<torch::Tensor> k_scales, c10::optional<torch::Tensor> v_scales,
+                     torch::Tensor page_table, torch::Tensor seq_lens, torch::Tensor cu_q,
+                     c10::optional<torch::Tensor> sinks, torch::Tensor out, int64_t hq, int64_t hkv,
+                     int64_t window, double scale, int64_t max_q_len, int64_t max_seq_len);
 void sample_tokens(torch::Tensor logits, torch::Tensor temperature, c10::optional<torch::Tensor> min_p,
                    torch::Tensor seeds, int64_t step, torch::Tensor tokens, torch::Tensor logprobs,
                    torch::Tensor entropy);
@@ -150,6 +161,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("decode_attention", &af3::decode_attention);
   m.def("kv_store", &af3::kv_store);
   m.def("kv_gather", &af3::kv_gather);
+  m.def("kv_store_fp8", &af3::kv_store_fp8, "new K/V rows -> e4m3 pages + e8m0 scale bytes");
+  m.def("kv_gather_fp8", &af3::kv_gather_fp8, "e4m3 page rows -> bf16 K/V rows");
+  m.def("paged_attention", &af3::paged_attention,
+        "attention of new tokens over bf16 or e4m3 cache pages");
   m.def("sample_tokens", &af3::sample_tokens);
   m.def("device_error", &af3::device_error_take,
         "Read and clear the current device's kernel error word (0 = no error).");

@@ -1,0 +1,62 @@
+// Device view of one layer's KV pages, shared by the kernels that read or write them.
+//
+// A pool is a tensor [pages, page_size, Hkv, D] of bf16 or of e4m3 codes whose rows of D
+// elements are contiguous; the other strides are free (e4m3 pools usually keep a KV head's rows
+// of a page together).  e4m3 pools come with one e8m0 byte b per row, [pages, Hkv, page_size]
+// with free strides: the row's values are code * 2^(b - 127), exact in bf16.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+namespace af3 {
+namespace paged {
+
+struct Pool {
+  uint8_t* k;
+  uint8_t* v;
+  uint8_t* ks;  // scale bytes, null for bf16 pages
+  uint8_t* vs;
+  // strides in bytes, the same for K and V
+  int64_t page, token, head;
+  int64_t s_page, s_head, s_token;
+  int num_pages, page_size, page_shift;  // page_shift: log2(page_size), -1 if not a power of two
+};
+
+__device__ __forceinline__ void split_slot(const Pool& p, uint32_t slot, uint32_t& page,
+                                           uint32_t& off) {
+  if (p.page_shift >= 0) {
+    page = slot >> p.page_shift;
+    off = slot & (uint32_t)(p.page_size - 1);
+  } else {
+    page = slot / (uint32_t)p.page_size;
+    off = slot - page * (uint32_t)p.page_size;
+  }
+}
+
+__device__ __forceinline__ float ex2a(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// 2^e for integer e in [-127, 127]; 2^-127 is a denormal.
+__device__ __forceinline__ float pow2i(int e) {
+  return e > -127 ? __uint_as_float((uint32_t)(e + 127) << 23) : __uint_as_float(0x00400000u);
+}
+
+// Two e4m3 codes (low byte first) -> f16 pair, exact.
+__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint16_t c) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(c));
+  return r;
+}
+
+__device__ __forceinline__ float2 f16x2_to_float2(uint32_t h) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+
+}  // namespace paged
+}  // namespace af3
