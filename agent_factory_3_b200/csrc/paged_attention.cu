@@ -1,7 +1,7 @@
 // Torch entry point of the attention over cache pages.
 #include "common.h"
 #include "host_utils.h"
-#include "paged_attention.cuh"
+#include "paged_attention.h"
 #include "paged_host.h"
 
 namespace af3 {
@@ -102,6 +102,12 @@ void paged_attention(torch::Tensor q, torch::Tensor k_pages, torch::Tensor v_pag
   a.window = (int)window;
   a.scale_log2 = (float)scale * kLog2e;
   auto stream = at::cuda::getCurrentCUDAStream();
+  max_q_len = std::max<int64_t>(max_q_len, 1);
+  max_seq_len = std::max<int64_t>(max_seq_len, 1);
+  if (std::min<int64_t>(max_q_len, a.T) * a.group <= kFewRows) {
+    launch_few(a, max_q_len, max_seq_len, stream);
+    return;
+  }
   const dim3 grid((unsigned)a.T, (unsigned)((hq + kRowThreads / 32 - 1) / (kRowThreads / 32)));
   if (a.p.ks != nullptr)
     paged_row_kernel<true><<<grid, kRowThreads, 0, stream>>>(a);

@@ -1,0 +1,622 @@
+// Attention over cache pages for few query rows a KV head (at most 32: decoding, short verify
+// blocks).  Reads every visible key and value once, so it is bound by memory: 4 KB (e4m3) or 8 KB
+// (bf16) of pages against ~500 instructions a warp for 32 keys.
+//
+// Work: one cluster of S CTAs per (sequence, KV head); the CTAs take contiguous parts of the keys
+// and join over distributed shared memory, so there is one launch, no workspace, and a fixed order
+// of every sum.  In a CTA each of the four warps runs on its own: every fourth block of 32 keys,
+// copied by cp.async into the warp's ring of kStages blocks, with its own running maximum, sum
+// and output, merged at the end.
+//
+// The matrix instructions (m16n8k16) run with the keys as M and the query rows as N, so 8 rows
+// waste nothing:
+//   S^T = K Q^T      M = 16 keys,  N = 8 rows, K = 64 dims in 4 steps
+//   O^T = V^T P^T    M = 16 dims (4 tiles), N = 8 rows, K = 16 keys
+// Index permutations make each load of a thread (group g = lane / 4, t = lane % 4) contiguous: in S
+// the thread feeds step s with dims 16t + 4s + {0,1} and 16t + 4s + {2,3} of key rows and query
+// rows; in O row g of dim tile i is dim 8g + 2i and row g + 8 is dim 8g + 2i + 1.  P^T comes out of
+// S^T's accumulator layout by movmatrix (an 8x8 transpose of 16-bit elements).
+//
+// e4m3 pages: codes are expanded to f16 (exact).  K's scale multiplies the score in fp32.  V's scale
+// is folded into P: P' = p * 2^(e - E) with E the largest V exponent seen by this warp so far; O is
+// rescaled when E grows.  The largest p is 2^10, so P' keeps f16's 11 bits down to 2^-24 of it.  The
+// query rows are brought to f16 after a power-of-two scaling to [1, 2), undone in fp32.
+// bf16 pages: K, V, Q as they are; P as the sum of two bf16 numbers (16 bits), since one alone would
+// cost as much precision as the rounding of the output.  The 8 more instructions of 32 keys hide
+// behind the copies.
+#include <cooperative_groups.h>
+
+#include "host_utils.h"
+#include "paged_attention.h"
+
+namespace cg = cooperative_groups;
+
+namespace af3 {
+namespace paged {
+
+constexpr int kWarps = 4;
+constexpr int kFewThreads = kWarps * 32;
+constexpr int kStages = 3;
+
+template <bool FP8>
+struct FewCfg {
+  static constexpr int kRowBytes = FP8 ? 64 : 128;
+  static constexpr int kStageBytes = 2 * 32 * kRowBytes;  // K then V
+  static constexpr int kRingBytes = kStages * kStageBytes;
+  static constexpr float kTop = FP8 ? 10.f : 0.f;  // the largest p of a row is 2^kTop
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
+  const int n = on ? 16 : 0;  // 0: the 16 bytes are filled with zeros and src is not read
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 r;
+  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(a));
+  return r;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+  uint2 r;
+  asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(a));
+  return r;
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
+  return r;
+}
+template <bool FP8>
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                         uint32_t b0, uint32_t b1) {
+  if constexpr (FP8) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  } else {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+}
+template <bool FP8>
+__device__ __forceinline__ uint32_t pack16x2(float lo, float hi) {
+  uint32_t r;
+  if constexpr (FP8)
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// Byte offset of 16-byte chunk c of key row r inside a block.  e4m3: two 64-byte rows share a
+// 128-byte line, chunks xored by twice the line's low bits; bf16: chunks xored by the row's low
+// bits.  Both leave the copies and both access patterns below free of bank conflicts.
+template <bool FP8>
+__device__ __forceinline__ uint32_t chunk_at(int r, int c) {
+  if constexpr (FP8) {
+    const int line = r >> 1;
+    return (uint32_t)(line * 128 + ((((r & 1) * 4 + c) ^ ((line & 3) << 1)) << 4));
+  } else {
+    return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4));
+  }
+}
+
+// Zeroes what is not finite in 16 bytes of V; true if there was something.
+template <bool FP8>
+__device__ __forceinline__ bool clear_nonfinite(uint32_t addr) {
+  uint4 w = lds128(addr);
+  uint32_t* x = reinterpret_cast<uint32_t*>(&w);
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t m = FP8 ? __vcmpeq4(x[i] & 0x7f7f7f7fu, 0x7f7f7f7fu) : __vcmpeq2(x[i] & 0x7f807f80u, 0x7f807f80u);
+    bad |= m != 0;
+    x[i] &= ~m;
+  }
+  if (bad)
+    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w) : "memory");
+  return bad;
+}
+
+// What lane l remembers of key l of a block in flight: K and V scale bytes, and whether it exists.
+constexpr uint32_t kThere = 1u << 16;
+
+template <bool FP8>
+__device__ __forceinline__ uint32_t issue_block(const Args& a, const int* table, int g, int base, int lo, int hi,
+                                                uint32_t dst) {
+  using C = FewCfg<FP8>;
+  const int lane = threadIdx.x & 31;
+  const int j = base + lane;
+  int64_t row = 0, sc = 0;
+  uint32_t info = 0;
+  const bool there = j >= lo && j < hi && key_row(a, table, j, g, row, sc);
+  if (there) {
+    info = kThere;
+    if constexpr (FP8) info |= (uint32_t)a.p.ks[sc] | ((uint32_t)a.p.vs[sc] << 8);
+  }
+  constexpr int kChunks = C::kRowBytes / 16, kRowsPer = 32 / kChunks;
+  // the rows' offsets travel by shuffle; a missing row has offset 0 and is filled with zeros.
+  // Nothing here waits for the scale bytes.
+  const uint32_t mask = __ballot_sync(0xffffffffu, there);
+  const int c = lane % kChunks;
+#pragma unroll
+  for (int i = 0; i < 32 / kRowsPer; ++i) {
+    const int r = i * kRowsPer + lane / kChunks;
+    const int64_t off = __shfl_sync(0xffffffffu, row, r) + c * 16;
+    const bool on = (mask >> r) & 1u;
+    const uint32_t d = dst + chunk_at<FP8>(r, c);
+    cp_async16(d, a.p.k + off, on);
+    cp_async16(d + 32 * C::kRowBytes, a.p.v + off, on);
+  }
+  return info;
+}
+
+template <bool FP8, int NT>
+__global__ void __launch_bounds__(kFewThreads, FP8 ? (NT == 1 ? 4 : NT == 2 ? 3 : 2) : 2) paged_few_kernel(const Args a, const int rows_per_tile,
+                                                                                const int splits) {
+  using C = FewCfg<FP8>;
+  constexpr int R = NT * 8;  // query rows of a tile
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float s_m[kWarps][R], s_l[kWarps][R];
+  __shared__ float c_m[R], c_l[R];
+  __shared__ int s_wide[kWarps];
+  float* c_o = reinterpret_cast<float*>(smem + kWarps * C::kRingBytes);  // [R][64], this CTA's part
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int grp = lane >> 2, tig = lane & 3;
+  const int rank = splits > 1 ? (int)blockIdx.x : 0;
+  const int g = blockIdx.y, b = blockIdx.z;
+  const Seq sq = load_seq(a, b);
+  const int tokens_per_tile = rows_per_tile / a.group;
+  const int* table = a.table + (int64_t)b * a.ld_table;
+  uint8_t* ring = smem + warp * C::kRingBytes;
+  const uint32_t ring_s = (uint32_t)__cvta_generic_to_shared(ring);
+
+  for (int tok0 = sq.t0; tok0 < sq.t1; tok0 += tokens_per_tile) {
+    const int ntok = min(tokens_per_tile, sq.t1 - tok0);
+    const int nrows = ntok * a.group;
+    const bool several = ntok > 1;  // rows differ in what they see
+    const int pos0 = sq.first + (tok0 - sq.t0);  // position of the tile's first token
+    // keys that any row of the tile may see
+    const int lo = a.window > 0 ? max(0, pos0 - a.window + 1) : 0;
+    const int hi = min(pos0 + ntok, sq.key_end);
+    const int blk0 = lo >> 5, blk1 = max((hi + 31) >> 5, blk0);
+    const int per = (blk1 - blk0 + splits - 1) / splits;
+    const int my0 = min(blk0 + rank * per, blk1), my1 = min(my0 + per, blk1);
+
+    // ---- query rows: thread (grp, tig) holds dims [16 tig, 16 tig + 16) of rows nt * 8 + grp
+    uint32_t qf[NT][8];
+    float smul[NT][2];  // rows nt * 8 + 2 tig + {0, 1}: softmax scale * log2(e) * the row's scaling
+    int rlo[NT][2], rhi[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int r = nt * 8 + grp;
+      uint4 w0 = make_uint4(0, 0, 0, 0), w1 = w0;
+      if (r < nrows) {
+        const uint4* src = reinterpret_cast<const uint4*>(
+            a.q + (int64_t)(tok0 + r / a.group) * a.ld_q + (int64_t)(g * a.group + r % a.group) * kD + 16 * tig);
+        w0 = src[0];
+        w1 = src[1];
+      }
+      const uint32_t w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+      float back = 1.f;
+      if constexpr (FP8) {
+        uint32_t mx = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) mx = max(mx, max(w[i] & 0x7fffu, (w[i] >> 16) & 0x7fffu));
+        mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        int e = (int)(mx >> 7) - 127;  // largest magnitude in [2^e, 2^(e+1))
+        if (e > 126 || e < -126) e = 0;  // zero, denormal, infinite or NaN rows: as they are
+        const float f = pow2i(-e);
+        back = pow2i(e);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float lo16 = __uint_as_float(w[i] << 16), hi16 = __uint_as_float(w[i] & 0xffff0000u);
+          qf[nt][i] = pack16x2<true>(lo16 * f, hi16 * f);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) qf[nt][i] = w[i];
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        smul[nt][c] = a.scale_log2 * __shfl_sync(0xffffffffu, back, (2 * tig + c) * 4);
+        const int rr = nt * 8 + 2 * tig + c;
+        const int p = pos0 + (rr < nrows ? rr / a.group : 0);
+        rhi[nt][c] = rr < nrows ? p : -1;
+        rlo[nt][c] = a.window > 0 ? p - a.window + 1 : 0;
+      }
+    }
+    // a block is full when every row sees all of it
+    const int full_lo = a.window > 0 ? pos0 + ntok - a.window : 0, full_hi = min(pos0 + 1, sq.key_end);
+
+    float m[NT][2], l[NT][2], o[NT][4][4];
+    int vmax = 0, vmin = 255;  // V's scale bytes seen (blocks of this warp); vmin skips zero rows
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      m[nt][0] = m[nt][1] = -INFINITY;
+      l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
+    }
+
+    uint32_t info[kStages];
+    const int first = my0 + warp;
+#pragma unroll
+    for (int s = 0; s < kStages - 1; ++s) {
+      info[s] = 0;
+      if (first + s * kWarps < my1)
+        info[s] = issue_block<FP8>(a, table, g, (first + s * kWarps) * 32, lo, hi, ring_s + s * C::kStageBytes);
+      cp_async_commit();
+    }
+    for (int blk = first; blk < my1; blk += kStages * kWarps) {
+#pragma unroll
+      for (int s = 0; s < kStages; ++s) {
+        const int cur = blk + s * kWarps;
+        if (cur >= my1) break;
+        {
+          constexpr int ahead = kStages - 1;
+          const int slot = (s + ahead) % kStages;
+          const int nxt = cur + ahead * kWarps;
+          __syncwarp();  // every lane has read the block that this slot held
+          if (nxt < my1) info[slot] = issue_block<FP8>(a, table, g, nxt * 32, lo, hi, ring_s + slot * C::kStageBytes);
+          cp_async_commit();
+        }
+        cp_async_wait<kStages - 1>();
+        __syncwarp();
+        const uint32_t kb = ring_s + s * C::kStageBytes, vb = kb + 32 * C::kRowBytes;
+        const int base = cur * 32;
+
+        // A value that is not finite would reach every row through 0 * inf.  Where rows differ in
+        // what they see, such values are taken out of the block (which leaves the rows that do not
+        // see them as they are), and the rows that see them are taken again at the end.
+        const bool full = base >= full_lo && base + 32 <= full_hi && __all_sync(0xffffffffu, info[s] & kThere);
+        uint32_t broken = 0;  // keys
+        if (several && !full) {
+          bool bad = false;
+#pragma unroll 1
+          for (int c = 0; c < C::kRowBytes / 16; ++c) bad |= clear_nonfinite<FP8>(vb + chunk_at<FP8>(lane, c));
+          broken = __ballot_sync(0xffffffffu, bad);
+          __syncwarp();
+        }
+
+        // ---- S^T, keys base + 16 mt + {grp, grp + 8}
+        float sc[2][NT][4];
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) sc[mt][nt][0] = sc[mt][nt][1] = sc[mt][nt][2] = sc[mt][nt][3] = 0.f;
+          const int r0 = mt * 16 + grp, r1 = r0 + 8;
+          if constexpr (FP8) {
+            const uint4 x = lds128(kb + chunk_at<true>(r0, tig)), y = lds128(kb + chunk_at<true>(r1, tig));
+            const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) {
+              const uint32_t a0 = e4m3x2_to_f16x2((uint16_t)xw[ks]), a2 = e4m3x2_to_f16x2((uint16_t)(xw[ks] >> 16));
+              const uint32_t a1 = e4m3x2_to_f16x2((uint16_t)yw[ks]), a3 = e4m3x2_to_f16x2((uint16_t)(yw[ks] >> 16));
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+                mma16816<true>(sc[mt][nt], a0, a1, a2, a3, qf[nt][2 * ks], qf[nt][2 * ks + 1]);
+            }
+          } else {
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+              const uint4 x = lds128(kb + chunk_at<false>(r0, 2 * tig + hf));
+              const uint4 y = lds128(kb + chunk_at<false>(r1, 2 * tig + hf));
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                mma16816<false>(sc[mt][nt], x.x, y.x, x.y, y.y, qf[nt][4 * hf], qf[nt][4 * hf + 1]);
+                mma16816<false>(sc[mt][nt], x.z, y.z, x.w, y.w, qf[nt][4 * hf + 2], qf[nt][4 * hf + 3]);
+              }
+            }
+          }
+        }
+        // ---- scales of this thread's four keys, masks
+        float vmul[4];
+        bool grew = false;
+        float shrink = 1.f;
+        if constexpr (FP8) {
+          const int mine = (info[s] & kThere) && !((broken >> lane) & 1u) ? (int)((info[s] >> 8) & 255u) : 0;
+          const int top = (int)__reduce_max_sync(0xffffffffu, (unsigned)mine);
+          vmin = min(vmin, mine > 0 ? mine : 255);
+          grew = top > vmax;
+          if (grew) {
+            shrink = pow2i(max(vmax - top, -127));
+            vmax = top;
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {  // keys grp + 8 k: mt = k / 2, accumulator half k % 2
+          const uint32_t inf = __shfl_sync(0xffffffffu, info[s], grp + 8 * k);
+          float kmul = 1.f;
+          if constexpr (FP8) {
+            kmul = pow2i((int)(inf & 255u) - 127);
+            vmul[k] = pow2i(max((int)((inf >> 8) & 255u) - vmax, -127));
+          }
+          const int key = base + grp + 8 * k;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              float& x = sc[k >> 1][nt][2 * (k & 1) + c];
+              x *= FP8 ? smul[nt][c] * kmul : smul[nt][c];
+              if (!full) {
+                if (!((inf & kThere) && key >= rlo[nt][c] && key <= rhi[nt][c]))
+                  x = -INFINITY;
+                else if ((broken >> (grp + 8 * k)) & 1u)
+                  l[nt][c] = __uint_as_float(0x7fc00000u);
+              }
+            }
+          }
+        }
+        // ---- running reference
+        bool need = false;
+        float mx[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            mx[nt][c] = fmaxf(fmaxf(sc[0][nt][c], sc[0][nt][2 + c]), fmaxf(sc[1][nt][c], sc[1][nt][2 + c]));
+            mx[nt][c] -= C::kTop;
+            need |= mx[nt][c] > m[nt][c];
+          }
+        }
+        if (__any_sync(0xffffffffu, need)) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              float x = mx[nt][c];
+              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+              if (x > m[nt][c]) {
+                const float f = ex2a(m[nt][c] - x);  // 0 from -inf
+                m[nt][c] = x;
+                l[nt][c] *= f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  o[nt][i][c] *= f;
+                  o[nt][i][2 + c] *= f;
+                }
+              }
+            }
+          }
+        }
+        if (FP8 && grew) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[nt][i][e] *= shrink;
+            }
+        }
+        // ---- P^T as B fragments
+        uint32_t pb[2][NT][2], pl[2][NT][2];  // pl: what pb's bf16 leaves out
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const float mu0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0], mu1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            float p0 = ex2a(sc[k >> 1][nt][2 * (k & 1)] - mu0);
+            float p1 = ex2a(sc[k >> 1][nt][2 * (k & 1) + 1] - mu1);
+            l[nt][0] += p0;
+            l[nt][1] += p1;
+            if constexpr (FP8) {
+              p0 *= vmul[k];
+              p1 *= vmul[k];
+            }
+            const uint32_t w = pack16x2<FP8>(p0, p1);
+            pb[k >> 1][nt][k & 1] = transpose8x8(w);
+            if constexpr (!FP8)
+              pl[k >> 1][nt][k & 1] = transpose8x8(
+                  pack16x2<false>(p0 - __uint_as_float(w << 16), p1 - __uint_as_float(w & 0xffff0000u)));
+          }
+        }
+        // ---- O^T += V^T P^T
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
+          const int r = mt * 16 + 2 * tig;
+          if constexpr (FP8) {
+            // dims [8 grp, 8 grp + 8): half of chunk grp / 2
+            const uint32_t in = (uint32_t)(grp & 1) * 8;
+            const uint2 x = lds64(vb + chunk_at<true>(r, grp >> 1) + in);
+            const uint2 y = lds64(vb + chunk_at<true>(r + 1, grp >> 1) + in);
+            const uint2 z = lds64(vb + chunk_at<true>(r + 8, grp >> 1) + in);
+            const uint2 u = lds64(vb + chunk_at<true>(r + 9, grp >> 1) + in);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              // bytes of dims 2i, 2i + 1 of two keys -> (key, key + 1) of dim 2i, then of dim 2i + 1
+              const uint32_t sel = (i & 1) ? 0x7362u : 0x5140u;
+              const uint32_t xy = __byte_perm(i < 2 ? x.x : x.y, i < 2 ? y.x : y.y, sel);
+              const uint32_t zu = __byte_perm(i < 2 ? z.x : z.y, i < 2 ? u.x : u.y, sel);
+              const uint32_t a0 = e4m3x2_to_f16x2((uint16_t)xy), a1 = e4m3x2_to_f16x2((uint16_t)(xy >> 16));
+              const uint32_t a2 = e4m3x2_to_f16x2((uint16_t)zu), a3 = e4m3x2_to_f16x2((uint16_t)(zu >> 16));
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) mma16816<true>(o[nt][i], a0, a1, a2, a3, pb[mt][nt][0], pb[mt][nt][1]);
+            }
+          } else {
+            const uint4 x = lds128(vb + chunk_at<false>(r, grp)), y = lds128(vb + chunk_at<false>(r + 1, grp));
+            const uint4 z = lds128(vb + chunk_at<false>(r + 8, grp)), u = lds128(vb + chunk_at<false>(r + 9, grp));
+            const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
+            const uint32_t zw[4] = {z.x, z.y, z.z, z.w}, uw[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t a0 = __byte_perm(xw[i], yw[i], 0x5410), a1 = __byte_perm(xw[i], yw[i], 0x7632);
+              const uint32_t a2 = __byte_perm(zw[i], uw[i], 0x5410), a3 = __byte_perm(zw[i], uw[i], 0x7632);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                mma16816<false>(o[nt][i], a0, a1, a2, a3, pb[mt][nt][0], pb[mt][nt][1]);
+                mma16816<false>(o[nt][i], a0, a1, a2, a3, pl[mt][nt][0], pl[mt][nt][1]);
+              }
+            }
+          }
+        }
+      }
+    }
+    cp_async_wait<0>();
+    __syncwarp();
+
+    // ---- this warp's part, normalised: (m, l, o / l)
+    float* w_o = reinterpret_cast<float*>(ring);  // [R][64] over the warp's ring
+    const float vscale = FP8 ? pow2i(vmax - 127) : 1.f;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float x = l[nt][c];
+        x += __shfl_xor_sync(0xffffffffu, x, 4);
+        x += __shfl_xor_sync(0xffffffffu, x, 8);
+        x += __shfl_xor_sync(0xffffffffu, x, 16);
+        const int r = nt * 8 + 2 * tig + c;
+        const float inv = x == 0.f ? 0.f : 1.f / x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          *reinterpret_cast<float2*>(w_o + r * kD + 8 * grp + 2 * i) =
+              make_float2(o[nt][i][c] * inv * vscale, o[nt][i][2 + c] * inv * vscale);
+        }
+        if (grp == 0) {
+          s_m[warp][r] = m[nt][c];
+          s_l[warp][r] = x;
+        }
+      }
+    }
+    if constexpr (FP8) {
+      const int least = (int)__reduce_min_sync(0xffffffffu, (unsigned)vmin);
+      if (lane == 0) s_wide[warp] = vmax - least > kWideRange;
+    }
+    __syncthreads();
+    // ---- join the warps: one warp a row, lane l has dims 2l, 2l + 1
+    bool wide = false;
+    if constexpr (FP8) {
+      if (several)
+        for (int w = 0; w < kWarps; ++w) wide |= s_wide[w] != 0;
+    }
+    for (int r = warp; r < nrows; r += kWarps) {
+      float mm = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, s_m[w][r]);
+      const float mu = mm == -INFINITY ? 0.f : mm;
+      float ll = 0.f, x = 0.f, y = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float f = s_l[w][r] * ex2a(s_m[w][r] - mu);
+        const float2 v = reinterpret_cast<const float2*>(smem + w * C::kRingBytes)[r * (kD / 2) + lane];
+        ll += f;
+        x = fmaf(f, v.x, x);
+        y = fmaf(f, v.y, y);
+      }
+      const float inv = ll == 0.f ? 0.f : 1.f / ll;
+      reinterpret_cast<float2*>(c_o)[r * (kD / 2) + lane] = make_float2(x * inv, y * inv);
+      if (lane == 0) {
+        c_m[r] = mm;
+        c_l[r] = wide ? __uint_as_float(0x7fc00000u) : ll;  // NaN: the row is taken key by key
+      }
+    }
+    if (splits > 1) cg::this_cluster().sync(); else __syncthreads();
+    // ---- join the CTAs; row r belongs to one warp of the cluster
+    for (int r = rank * kWarps + warp; r < nrows; r += splits * kWarps) {
+      const int h = g * a.group + r % a.group, t = tok0 + r / a.group;
+      const float sk = a.sinks != nullptr ? a.sinks[h] * kLog2e : -INFINITY;
+      float mc = -INFINITY, lc = 0.f;
+      if (lane < splits) {
+        mc = splits > 1 ? *cg::this_cluster().map_shared_rank(&c_m[r], lane) : c_m[r];
+        lc = splits > 1 ? *cg::this_cluster().map_shared_rank(&c_l[r], lane) : c_l[r];
+      }
+      float top = fmaxf(mc, sk);
+#pragma unroll
+      for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+      const float tu = top == -INFINITY ? 0.f : top;
+      const float f = lc * ex2a(mc - tu);
+      float den = f;
+#pragma unroll
+      for (int x = 16; x > 0; x >>= 1) den += __shfl_xor_sync(0xffffffffu, den, x);
+      den += ex2a(sk - tu);
+      float x = 0.f, y = 0.f;
+      for (int c = 0; c < splits; ++c) {
+        const float fc = __shfl_sync(0xffffffffu, f, c);
+        const float2* src = reinterpret_cast<const float2*>(c_o) + r * (kD / 2) + lane;
+        if (splits > 1) src = cg::this_cluster().map_shared_rank(src, c);
+        const float2 v = *src;
+        x = fmaf(fc, v.x, x);
+        y = fmaf(fc, v.y, y);
+      }
+      const float inv = den == 0.f ? 0.f : 1.f / den;
+      x *= inv;
+      y *= inv;
+      // Rows that see a value that is not finite (an infinity comes out of the two halves of P as
+      // NaN), and tiles of too wide a range: key by key.
+      const bool bad = !(fabsf(x) < INFINITY && fabsf(y) < INFINITY);
+      if (__any_sync(0xffffffffu, bad)) {
+        const int p = pos0 + r / a.group;
+        warp_row<FP8>(a, table, t, h, a.window > 0 ? max(0, p - a.window + 1) : 0, min(p + 1, sq.key_end), x, y);
+      }
+      reinterpret_cast<__nv_bfloat162*>(a.out + (int64_t)t * a.ld_out + (int64_t)h * kD)[lane] =
+          __floats2bfloat162_rn(x, y);
+    }
+    // parts may be overwritten (next tile) or go away (exit) only when every CTA has read them
+    if (splits > 1) cg::this_cluster().sync(); else __syncthreads();
+  }
+}
+
+template <bool FP8, int NT>
+static void launch_few_nt(const Args& a, int rows_per_tile, int splits, cudaStream_t stream) {
+  using C = FewCfg<FP8>;
+  constexpr int smem = kWarps * C::kRingBytes + NT * 8 * kD * 4;
+  static_assert(NT * 8 * kD * 4 <= C::kRingBytes, "a warp's part has to fit its ring");
+  auto kern = paged_few_kernel<FP8, NT>;
+  static bool ready[64] = {};
+  int dev;
+  AF3_CUDA_CHECK(cudaGetDevice(&dev));
+  if (!ready[dev]) {
+    AF3_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    AF3_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    ready[dev] = true;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)splits, (unsigned)a.hkv, (unsigned)a.B);
+  cfg.blockDim = dim3(kFewThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim = {(unsigned)splits, 1, 1};
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  AF3_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, a, rows_per_tile, splits));
+}
+
+template <bool FP8>
+static void launch_few_t(const Args& a, int max_q, int splits, cudaStream_t stream) {
+  const int want = std::max(std::min(max_q, kFewRows / a.group), 1) * a.group;  // rows of a tile
+  if (want <= 8)
+    launch_few_nt<FP8, 1>(a, want, splits, stream);
+  else if (want <= 16)
+    launch_few_nt<FP8, 2>(a, want, splits, stream);
+  else
+    launch_few_nt<FP8, 4>(a, want, splits, stream);
+}
+
+void launch_few(const Args& a, int64_t max_q, int64_t max_len, cudaStream_t stream) {
+  // Keys are split until the machine has about four CTAs an SM to choose from, as long as a part
+  // has 256 keys (two blocks a warp); 16 CTAs is the largest cluster.
+  const int64_t keys = a.window > 0 ? std::min<int64_t>(max_len, a.window + max_q) : max_len;
+  const int64_t items = (int64_t)a.B * a.hkv, enough = 4 * (int64_t)num_sms();
+  int splits = 1;
+  while (splits < 16 && items * splits < enough && keys >= 512 * splits) splits *= 2;
+  if (a.p.ks != nullptr)
+    launch_few_t<true>(a, (int)std::min<int64_t>(max_q, kFewRows), splits, stream);
+  else
+    launch_few_t<false>(a, (int)std::min<int64_t>(max_q, kFewRows), splits, stream);
+}
+
+}  // namespace paged
+}  // namespace af3
