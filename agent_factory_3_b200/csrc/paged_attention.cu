@@ -5,40 +5,6 @@
 #include "paged_host.h"
 
 namespace af3 {
-namespace paged {
-
-constexpr int kRowThreads = 128;
-
-// The largest b with cu[b] <= t (a.B when t is past the last row).
-__device__ __forceinline__ int seq_of_row(const Args& a, int t) {
-  int lo = 0, hi = a.B;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (a.cu[mid] <= t) lo = mid; else hi = mid - 1;
-  }
-  return lo;
-}
-
-// One warp per (row, head).
-template <bool FP8>
-__global__ void __launch_bounds__(kRowThreads) paged_row_kernel(const Args a) {
-  const int t = blockIdx.x;
-  const int h = blockIdx.y * (kRowThreads / 32) + threadIdx.x / 32;
-  if (h >= a.hq) return;
-  const int b = seq_of_row(a, t);
-  if (b >= a.B) return;
-  const Seq s = load_seq(a, b);
-  if (t < s.t0 || t >= s.t1) return;
-  const int pos = s.first + (t - s.t0);
-  const int lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
-  const int hi = min(pos + 1, s.key_end);
-  float o0, o1;
-  warp_row<FP8>(a, a.table + (int64_t)b * a.ld_table, t, h, lo, hi, o0, o1);
-  reinterpret_cast<__nv_bfloat162*>(a.out + (int64_t)t * a.ld_out + (int64_t)h * kD)[threadIdx.x & 31] =
-      __floats2bfloat162_rn(o0, o1);
-}
-
-}  // namespace paged
 
 void paged_attention(torch::Tensor q, torch::Tensor k_pages, torch::Tensor v_pages,
                      c10::optional<torch::Tensor> k_scales, c10::optional<torch::Tensor> v_scales,
@@ -81,6 +47,7 @@ void paged_attention(torch::Tensor q, torch::Tensor k_pages, torch::Tensor v_pag
                   sinks->numel() == hq && sinks->is_contiguous(),
               "sinks must be fp32 [Hq] on q's device");
   AF3_CHECK(window >= 0 && window < INT32_MAX, "window must not be negative");
+  AF3_CHECK(scale > 0, "scale must be positive");
   AF3_CHECK(q.size(0) < (int64_t(1) << 30) && seq_lens.size(0) < 65536, "batch too large");
   const c10::cuda::CUDAGuard guard(q.device());
   if (q.size(0) == 0 || seq_lens.size(0) == 0) return;
@@ -104,16 +71,10 @@ void paged_attention(torch::Tensor q, torch::Tensor k_pages, torch::Tensor v_pag
   auto stream = at::cuda::getCurrentCUDAStream();
   max_q_len = std::max<int64_t>(max_q_len, 1);
   max_seq_len = std::max<int64_t>(max_seq_len, 1);
-  if (std::min<int64_t>(max_q_len, a.T) * a.group <= kFewRows) {
+  if (std::min<int64_t>(max_q_len, a.T) * a.group <= kFewRows)
     launch_few(a, max_q_len, max_seq_len, stream);
-    return;
-  }
-  const dim3 grid((unsigned)a.T, (unsigned)((hq + kRowThreads / 32 - 1) / (kRowThreads / 32)));
-  if (a.p.ks != nullptr)
-    paged_row_kernel<true><<<grid, kRowThreads, 0, stream>>>(a);
   else
-    paged_row_kernel<false><<<grid, kRowThreads, 0, stream>>>(a);
-  AF3_CUDA_CHECK(cudaGetLastError());
+    launch_chunk(a, max_q_len, max_seq_len, stream);
 }
 
 }  // namespace af3

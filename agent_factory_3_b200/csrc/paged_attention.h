@@ -15,5 +15,9 @@ constexpr int kWideRange = 14;
 // At most kFewRows query rows a KV head and sequence: memory-bound, split over the keys.
 void launch_few(const Args& a, int64_t max_q, int64_t max_len, cudaStream_t stream);
 
+// Any number of rows, at most 128 query heads a KV head: tensor cores, split over the keys when
+// there are few rows.
+void launch_chunk(const Args& a, int64_t max_q, int64_t max_len, cudaStream_t stream);
+
 }  // namespace paged
 }  // namespace af3

@@ -1,0 +1,840 @@
+// Attention over cache pages for many query rows a KV head (prefill chunks, longer verify blocks),
+// on the fifth-generation tensor cores.
+//
+// One CTA per (span of up to 2 x 128 query rows, KV head); a row is a (token, query head of the
+// group) pair, floor(128 / group) tokens a tile, so the whole group shares every K/V block.  Few
+// spans over a long context are split: the CTAs of a cluster take parts of the keys and join over
+// distributed shared memory.
+//   warps 0-3    loaders: rows of 128-key blocks by cp.async (any page size and stride), three
+//                blocks ahead, expanded into 128B-swizzled f16 tiles
+//   warps 4-11   softmax, one warpgroup per 128-row tile: thread t owns query row t
+//   warp 12      tcgen05 issuer: S = Q K^T (M 128, N 128, K 64) of the next block is issued before
+//                O += P V (M 128, N 64, K 128, P from TMEM) of this one
+// TMEM columns: S[A] 0, S[B] 128, P[A] 256, P[B] 320 (f16 pairs), O[A] 384, O[B] 448.
+//
+// P and V enter the second product as f16: bf16's 8 bits for P would cost as much precision as the
+// rounding of the output.  V is scaled by a power of two that follows the largest magnitude the
+// CTA has loaded (its unit 2^u; O is rescaled when u grows), so that f16 holds all of it:
+//   e4m3 pages: V' = code * 2^(e - u), K' = code * 2^(e - ek) with ek the block's largest exponent;
+//               both exact while a key's exponent is within kWideRange of the largest
+//   bf16 pages: V' = v * 2^-u with the largest |V'| in [2^8, 2^9); K and Q stay bf16
+// The softmax reference moves only when a score passes it by 2^8; P is in (0, 2^14].  The row sum
+// adds the rounded P, so that a row that one key dominates comes out as that key's value.
+//
+// Rows that do not see a value must not meet it as 0 * inf: blocks that are not fully visible to
+// the whole span have such values cleared by the loaders and their keys reported; rows that do see
+// one, and spans of too wide a range, are taken key by key at the end.
+#include <cooperative_groups.h>
+
+#include "common.h"
+#include "host_utils.h"
+#include "paged_attention.h"
+#include "sm100.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace af3 {
+namespace paged {
+
+constexpr int kChunkThreads = 512;
+constexpr int kBK = 128;         // keys of a block
+constexpr int kST = 4;           // f16 K/V stages
+constexpr int kRaw = 3;          // raw blocks in flight
+constexpr int kTile = kBK * kD * 2;  // 16 KB: a 16-bit K, V or Q tile; also a raw block
+constexpr uint32_t kColS = 0, kColP = 256, kColO = 384;
+constexpr float kTopLog2 = 10.f, kGrowLog2 = 0.f;
+
+struct ChunkSmem {
+  static constexpr int Q = 0;                    // 2 tiles
+  static constexpr int K = Q + 2 * kTile;        // kST tiles
+  static constexpr int V = K + kST * kTile;      // kST tiles
+  static constexpr int RAW = V + kST * kTile;    // kRaw raw blocks: own 16-byte pieces of each loader thread
+  static constexpr int INFO = RAW + kRaw * kTile;
+  static constexpr int TOTAL = INFO + 2048;
+};
+
+struct StageInfo {
+  uint32_t there[4];   // keys that exist and lie in the span's range
+  uint32_t broken[4];  // keys whose V is not finite (cleared), in blocks not seen by every row
+  float kmul;          // 2^ek
+  int unit;            // V' is in units of 2^unit
+};
+
+struct ChunkBars {
+  uint64_t q_full, kv_full[kST], kv_empty[kST], s_full[2], s_free[2], p_full[2], o_ready[2];
+  uint32_t tmem;
+  int abort_flag;
+  int wide;
+  uint32_t red[2][4][2];
+  StageInfo info[kST];
+  float row_m[256], row_l[256];
+};
+static_assert(sizeof(ChunkBars) <= 4096, "");
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool on) {
+  const int n = on ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ uint4 lds4(uint32_t a) {
+  uint4 r;
+  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(a));
+  return r;
+}
+// 16-byte chunk c of row r of a 128B-swizzled tile of 128-byte rows
+__device__ __forceinline__ uint32_t sw128(int r, int c) { return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4)); }
+
+__device__ __forceinline__ uint64_t pk2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void upk2(uint64_t v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t h2_of(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// s0 += low half of w, s1 += high half
+__device__ __forceinline__ void add_h2(float& s0, float& s1, uint32_t w) {
+  asm("{\n.reg .f16 l, h;\nmov.b32 {l, h}, %2;\nadd.rn.f32.f16 %0, l, %0;\nadd.rn.f32.f16 %1, h, %1;\n}"
+      : "+f"(s0), "+f"(s1)
+      : "r"(w));
+}
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// f16 pair (2^e, 2^e) for e <= 0; 0 below f16's range
+__device__ __forceinline__ uint32_t h2_pow2(int e) {
+  const uint32_t h = e >= -14 ? (uint32_t)(e + 15) << 10 : e >= -24 ? 1u << (e + 24) : 0u;
+  return h | (h << 16);
+}
+
+// The keys a tile's rows see, and its blocks within this CTA's part.
+struct Tile {
+  int tok0, ntok, pos0;
+  int jlo, jhi;  // blocks, absolute; empty when jhi <= jlo
+};
+
+__device__ __forceinline__ Tile make_tile(const Args& a, const Seq& s, int tok0, int tokens, int kv_lo, int b0, int b1) {
+  Tile t;
+  t.tok0 = tok0;
+  t.ntok = max(0, min(tokens, s.t1 - tok0));
+  t.pos0 = s.first + (tok0 - s.t0);
+  const int lo = a.window > 0 ? max(0, t.pos0 - a.window + 1) : 0;
+  const int hi = min(t.pos0 + t.ntok, s.key_end);
+  t.jlo = t.jhi = b0;
+  if (t.ntok > 0 && hi > lo) {
+    t.jlo = max(b0, (lo - kv_lo) / kBK);
+    t.jhi = min(b1, (hi - 1 - kv_lo) / kBK + 1);
+  }
+  return t;
+}
+
+// The sequence of a span slot: the largest b with cu[b] / span + b <= slot (slots of b are at
+// least as many as its spans, see launch_chunk).
+__device__ __forceinline__ int seq_of_slot(const Args& a, int span, int slot) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, n = a.B;
+  while (n > 1) {
+    const int step = (n + 31) / 32;
+    const int i = lane * step;
+    const bool le = i < n && min(max(a.cu[lo + i], 0), a.T) / span + (lo + i) <= slot;
+    const int cnt = max(__popc(__ballot_sync(0xffffffffu, le)), 1);
+    lo += (cnt - 1) * step;
+    n = min(step, n - (cnt - 1) * step);
+  }
+  return lo;
+}
+
+// ------------------------------------------------------------------------------- issuer
+struct Issue {
+  int jlo, jhi, n_s, n_pv;
+};
+
+template <bool FP8, int X>
+__device__ __forceinline__ bool issue_s(Issue& t, int j, int st, uint32_t tmem, uint32_t sq, uint32_t sk0, ChunkBars* b,
+                                        int* err) {
+  if (j < t.jlo || j >= t.jhi) return true;
+  if (t.n_s > 0 && !mbar_wait(&b->s_free[X], (t.n_s - 1) & 1, err, &b->abort_flag)) return false;
+  tc_fence_after();
+  constexpr uint32_t idesc = FP8 ? make_idesc_f16(128, kBK, false, false) : make_idesc_bf16(128, kBK, false, false);
+  const uint32_t q = sq + X * kTile, k = sk0 + st * kTile;
+#pragma unroll
+  for (int kk = 0; kk < kD / 16; ++kk)
+    umma_f16(tmem + kColS + X * kBK, make_smem_desc(q + kk * 32, 16, 1024, kLayoutSW128),
+             make_smem_desc(k + kk * 32, 16, 1024, kLayoutSW128), idesc, kk > 0);
+  umma_commit(&b->s_full[X]);
+  ++t.n_s;
+  return true;
+}
+
+template <int X>
+__device__ __forceinline__ bool issue_pv(Issue& t, int j, int st, uint32_t tmem, uint32_t sv0, ChunkBars* b, int* err) {
+  if (j < t.jlo || j >= t.jhi) return true;
+  if (!mbar_wait(&b->p_full[X], t.n_pv & 1, err, &b->abort_flag)) return false;
+  tc_fence_after();
+  constexpr uint32_t idesc = make_idesc_f16(128, kD, false, true);
+  const uint32_t v = sv0 + st * kTile;
+  const uint32_t first = t.n_pv > 0 ? 1u : 0u;
+#pragma unroll
+  for (int kk = 0; kk < kBK / 16; ++kk)
+    umma_f16_tmem_a(tmem + kColO + X * kD, tmem + kColP + X * 64 + kk * 8,
+                    make_smem_desc(v + kk * 2048, 8192, 1024, kLayoutSW128), idesc, kk > 0 ? 1u : first);
+  umma_commit(&b->o_ready[X]);
+  ++t.n_pv;
+  return true;
+}
+
+// ------------------------------------------------------------------------------- loader
+// Rows of a block: warp w has keys [32 w, 32 w + 32); lane l looks up key 32 w + l.
+struct Ahead {
+  uint32_t there;
+  int64_t scale;  // offset of the lane's scale bytes
+};
+
+template <bool FP8>
+__device__ __forceinline__ Ahead load_block(const Args& a, const int* table, int g, int k0, int lo, int hi, int w, int lane,
+                                            uint32_t raw, uint32_t kdst) {
+  const int j = k0 + 32 * w + lane;
+  int64_t row = 0, sc = 0;
+  const bool on = j >= lo && j < hi && key_row(a, table, j, g, row, sc);
+  Ahead h;
+  h.there = __ballot_sync(0xffffffffu, on);
+  h.scale = sc;
+  const uint32_t own = raw + (32 * w + lane) * 16;
+  if constexpr (FP8) {  // K pieces 0-3, V pieces 4-7, 16 codes each
+    const int c = lane & 3;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = 8 * i + (lane >> 2);
+      const int64_t off = __shfl_sync(0xffffffffu, row, r) + c * 16;
+      const bool there = (h.there >> r) & 1u;
+      cp16(own + i * 2048, a.p.k + off, there);
+      cp16(own + (4 + i) * 2048, a.p.v + off, there);
+    }
+  } else {  // K straight into its tile, V pieces 0-7
+    const int c = lane & 7;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = 4 * i + (lane >> 3);
+      const int64_t off = __shfl_sync(0xffffffffu, row, r) + c * 16;
+      const bool there = (h.there >> r) & 1u;
+      cp16(kdst + sw128(32 * w + r, c), a.p.k + off, there);
+      cp16(own + i * 2048, a.p.v + off, there);
+    }
+  }
+  return h;
+}
+
+__device__ __forceinline__ void st4(uint32_t addr, uint32_t x, uint32_t y, uint32_t z, uint32_t u) {
+  st_shared_v4(addr, x, y, z, u);
+}
+
+// 16 e4m3 codes -> 16 f16 scaled by mul, into chunks 2c and 2c + 1 of row r.
+__device__ __forceinline__ void expand16(uint32_t tile, int r, int c, const uint4& w, uint32_t mul) {
+  const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+  uint32_t o[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    o[2 * i] = hmul2(e4m3x2_to_f16x2((uint16_t)x[i]), mul);
+    o[2 * i + 1] = hmul2(e4m3x2_to_f16x2((uint16_t)(x[i] >> 16)), mul);
+  }
+  st4(tile + sw128(r, 2 * c), o[0], o[1], o[2], o[3]);
+  st4(tile + sw128(r, 2 * c + 1), o[4], o[5], o[6], o[7]);
+}
+
+template <bool FP8>
+__global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Args a, const int tokens, const int splits,
+                                                                      int* err) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ ChunkBars bars;
+  ChunkBars* b = &bars;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = splits > 1 ? (int)(blockIdx.x % (unsigned)splits) : 0;
+  const int slots = gridDim.x / splits;
+  const int slot = slots - 1 - (int)(blockIdx.x / (unsigned)splits);  // the longest spans of a sequence first
+  const int g = blockIdx.y;
+  const int span = 2 * tokens;
+  const int sb = seq_of_slot(a, span, slot);
+  const Seq sq = load_seq(a, sb);
+  const int idx = slot - (sq.t0 / span + sb);
+  // (64-bit: a slot far past the sequence's rows must not wrap)
+  const int64_t tok64 = (int64_t)sq.t0 + (int64_t)idx * span;
+  if (idx < 0 || tok64 >= sq.t1) return;  // the whole cluster
+  const int tok0 = (int)tok64;
+  const int ntok = min(span, sq.t1 - tok0);
+  const int pos0 = sq.first + (tok0 - sq.t0);
+  const int lo = a.window > 0 ? max(0, pos0 - a.window + 1) : 0;
+  const int hi = max(min(pos0 + ntok, sq.key_end), lo);
+  const int nb = (hi - lo + kBK - 1) / kBK;
+  const int per = (nb + splits - 1) / splits;
+  const int b0 = min(rank * per, nb), b1 = min(b0 + per, nb);
+  const int* table = a.table + (int64_t)sb * a.ld_table;
+  const Tile tl[2] = {make_tile(a, sq, tok0, tokens, lo, b0, b1), make_tile(a, sq, tok0 + tokens, tokens, lo, b0, b1)};
+
+  if (warp == 0 && lane == 0) {
+    mbar_init(&b->q_full, 8);
+    for (int s = 0; s < kST; ++s) {
+      mbar_init(&b->kv_full[s], 4);
+      mbar_init(&b->kv_empty[s], 1);
+    }
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(&b->s_full[x], 1);
+      mbar_init(&b->s_free[x], 4);
+      mbar_init(&b->p_full[x], 4);
+      mbar_init(&b->o_ready[x], 1);
+    }
+    b->abort_flag = 0;
+    b->wide = 0;
+    fence_barrier_init();
+  }
+  if (warp == 13) {
+    tmem_alloc(&b->tmem, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = b->tmem;
+  const uint32_t sbase = smem_u32(smem);
+
+  // registers (launch: 512 x 128): loaders 88, softmax 2 x 192, issuer 40: 512 x 128 in all
+  if (warp < 4) {
+    setmaxnreg_dec<88>();
+    const int w = warp;
+    // a block is seen in full by every row of the span when it lies in [full_lo, full_hi)
+    const int full_lo = a.window > 0 ? pos0 + ntok - a.window : 0, full_hi = min(pos0 + 1, sq.key_end);
+    uint32_t top = 0;  // V: largest e8m0 byte (e4m3) or biased exponent (bf16) so far
+    bool dead = false;
+    Ahead ah[kRaw];
+    uint32_t scale_bytes = 0;  // of the next block to expand: K | V << 8
+    auto fetch_scales = [&](const Ahead& h) {
+      scale_bytes = 0;
+      if (FP8 && ((h.there >> lane) & 1u)) scale_bytes = (uint32_t)a.p.ks[h.scale] | ((uint32_t)a.p.vs[h.scale] << 8);
+    };
+#pragma unroll
+    for (int i = 0; i < kRaw; ++i) {
+      ah[i].there = 0;
+      ah[i].scale = 0;
+      if (b0 + i < b1)
+        ah[i] = load_block<FP8>(a, table, g, lo + (b0 + i) * kBK, lo, hi, w, lane, sbase + ChunkSmem::RAW + i * kTile,
+                                sbase + ChunkSmem::K + i * kTile);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    fetch_scales(ah[0]);
+    int raw_slot = 0;
+    for (int j = b0; j < b1; ++j) {
+      const int n = j - b0, st = n % kST;
+      const uint32_t raw = sbase + ChunkSmem::RAW + raw_slot * kTile;
+      const uint32_t own = raw + (32 * w + lane) * 16;
+      const uint32_t ktile = sbase + ChunkSmem::K + st * kTile, vtile = sbase + ChunkSmem::V + st * kTile;
+      asm volatile("cp.async.wait_group %0;" ::"n"(kRaw - 1) : "memory");
+      const int k0 = lo + j * kBK;
+      const uint32_t there = ah[0].there;
+      const bool partial = k0 < full_lo || k0 + kBK > full_hi;
+      uint32_t broken = 0;  // keys of this warp
+      uint4 v[FP8 ? 4 : 8];
+#pragma unroll
+      for (int i = 0; i < (FP8 ? 4 : 8); ++i) v[i] = lds4(own + ((FP8 ? 4 : 0) + i) * 2048);
+      // ---- exponents of this block: largest K, largest V, smallest nonzero of each
+      uint32_t kmax = 0, vmax = 0, kmin = 255, vmin = 255;
+      if constexpr (FP8) {
+        if (partial) {
+          bool bad[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t* x = reinterpret_cast<uint32_t*>(&v[i]);
+            bad[i] = false;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t m = __vcmpeq4(x[e] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+              bad[i] |= m != 0;
+              x[e] &= ~m;
+            }
+            uint32_t q = __ballot_sync(0xffffffffu, bad[i]);  // lanes 4 r .. 4 r + 3: key 8 i + r
+            q |= q >> 1;
+            q |= q >> 2;
+            q &= 0x11111111u;
+#pragma unroll
+            for (int r = 0; r < 8; ++r) broken |= ((q >> (4 * r)) & 1u) << (8 * i + r);
+          }
+        }
+        uint32_t kb = scale_bytes & 255u, vb = (scale_bytes >> 8) & 255u;
+        if (kb == 255u) kb = 0;
+        if (((broken >> lane) & 1u) || vb == 255u) vb = 0;
+        kmax = __reduce_max_sync(0xffffffffu, kb);
+        vmax = __reduce_max_sync(0xffffffffu, vb);
+        kmin = __reduce_min_sync(0xffffffffu, kb ? kb : 255u);
+        vmin = __reduce_min_sync(0xffffffffu, vb ? vb : 255u);
+      } else {
+        uint32_t all = 0, least = 255;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          uint32_t* x = reinterpret_cast<uint32_t*>(&v[i]);
+          uint32_t m2 = __vmaxu2(__vmaxu2(x[0] & 0x7fff7fffu, x[1] & 0x7fff7fffu),
+                                 __vmaxu2(x[2] & 0x7fff7fffu, x[3] & 0x7fff7fffu));
+          uint32_t m = max(m2 & 0xffffu, m2 >> 16);
+          if (__any_sync(0xffffffffu, m >= 0x7f80u)) {  // something is not finite
+            m = 0;
+            bool bad = false;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t f = __vcmpeq2(x[e] & 0x7f807f80u, 0x7f807f80u);
+              const uint32_t fin = x[e] & ~f & 0x7fff7fffu;
+              m = max(m, max(fin & 0xffffu, fin >> 16));
+              bad |= f != 0;
+              if (partial) x[e] &= ~f;
+            }
+            uint32_t q = __ballot_sync(0xffffffffu, bad && partial);  // lanes 8 r .. 8 r + 7: key 4 i + r
+#pragma unroll
+            for (int r = 0; r < 4; ++r) broken |= (((q >> (8 * r)) & 255u) ? 1u : 0u) << (4 * i + r);
+          }
+          m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+          m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+          m = max(m, __shfl_xor_sync(0xffffffffu, m, 4));
+          all = max(all, m >> 7);
+          if (m >> 7) least = min(least, m >> 7);
+        }
+        vmax = __reduce_max_sync(0xffffffffu, all);
+        vmin = __reduce_min_sync(0xffffffffu, least);
+      }
+      if (lane == 0) b->red[n & 1][w][0] = kmax | (vmax << 8) | (kmin << 16) | (vmin << 24);
+      named_barrier_sync(1, 128);
+      uint32_t kt = 0, vt = 0, kl = 255, vl = 255;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t x = b->red[n & 1][i][0];
+        kt = max(kt, x & 255u);
+        vt = max(vt, (x >> 8) & 255u);
+        kl = min(kl, (x >> 16) & 255u);
+        vl = min(vl, x >> 24);
+      }
+      top = max(top, vt);
+      if (threadIdx.x == 0 && ((kl != 255u && kt - kl > (uint32_t)kWideRange) || (vl != 255u && (int)(top - vl) > kWideRange)))
+        b->wide = 1;
+      if (!dead && n >= kST && !mbar_wait(&b->kv_empty[st], ((n / kST) & 1) ^ 1, err, &b->abort_flag)) dead = true;
+      // ---- expand into the f16 tiles
+      if constexpr (FP8) {
+        const int c = lane & 3;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = 8 * i + (lane >> 2);
+          const uint32_t sc = __shfl_sync(0xffffffffu, scale_bytes, r);
+          const uint4 k = lds4(own + i * 2048);
+          expand16(ktile, 32 * w + r, c, k, h2_pow2(min((int)(sc & 255u) - (int)kt, 0)));
+          expand16(vtile, 32 * w + r, c, v[i], h2_pow2(min((int)((sc >> 8) & 255u) - (int)top, 0)));
+        }
+      } else {
+        // largest |V'| in [2^8, 2^9): v * 2^(135 - top)
+        const float f = pow2i(135 - (int)max(top, 9u));
+        const uint64_t ff = pk2(f, f);
+        const int c = lane & 7;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t x[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+          uint32_t o[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float p0, p1;
+            upk2(fma2(pk2(__uint_as_float(x[e] << 16), __uint_as_float(x[e] & 0xffff0000u)), ff, pk2(0.f, 0.f)), p0, p1);
+            o[e] = h2_of(p0, p1);
+          }
+          st4(vtile + sw128(32 * w + 4 * i + (lane >> 3), c), o[0], o[1], o[2], o[3]);
+        }
+      }
+      if (lane == 0) {
+        b->info[st].there[w] = there;
+        b->info[st].broken[w] = broken;
+      }
+      if (threadIdx.x == 0) {
+        b->info[st].kmul = FP8 ? pow2i((int)kt - 127) : 1.f;
+        b->info[st].unit = FP8 ? (int)top - 127 : (int)max(top, 9u) - 135;
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&b->kv_full[st]);
+      // ---- refill
+#pragma unroll
+      for (int i = 0; i < kRaw - 1; ++i) ah[i] = ah[i + 1];
+      ah[kRaw - 1].there = 0;
+      if (j + kRaw < b1) {
+        const int ns = (n + kRaw) % kST;
+        if (!FP8 && !dead && n + kRaw >= kST &&   // K goes straight into its tile
+            !mbar_wait(&b->kv_empty[ns], (((n + kRaw) / kST) & 1) ^ 1, err, &b->abort_flag))
+          dead = true;
+        ah[kRaw - 1] = load_block<FP8>(a, table, g, lo + (j + kRaw) * kBK, lo, hi, w, lane, raw,
+                                       sbase + ChunkSmem::K + ns * kTile);
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      fetch_scales(ah[0]);
+      raw_slot = raw_slot + 1 == kRaw ? 0 : raw_slot + 1;
+    }
+  } else if (warp >= 12) {
+    setmaxnreg_dec<40>();
+    if (warp == 12 && b1 > b0 && elect_one_sync()) {
+      const uint32_t sqa = sbase + ChunkSmem::Q, sk0 = sbase + ChunkSmem::K, sv0 = sbase + ChunkSmem::V;
+      Issue ta{tl[0].jlo, tl[0].jhi, 0, 0}, tb{tl[1].jlo, tl[1].jhi, 0, 0};
+      bool ok = mbar_wait(&b->q_full, 0, err, &b->abort_flag) && mbar_wait(&b->kv_full[0], 0, err, &b->abort_flag);
+      ok = ok && issue_s<FP8, 0>(ta, b0, 0, tmem, sqa, sk0, b, err) && issue_s<FP8, 1>(tb, b0, 0, tmem, sqa, sk0, b, err);
+      for (int j = b0; ok && j < b1; ++j) {
+        const int n = j - b0, st = n % kST, sn = (n + 1) % kST;
+        const bool next = j + 1 < b1;
+        if (next) ok = mbar_wait(&b->kv_full[sn], ((n + 1) / kST) & 1, err, &b->abort_flag);
+        if (ok && next) ok = issue_s<FP8, 0>(ta, j + 1, sn, tmem, sqa, sk0, b, err);
+        ok = ok && issue_pv<0>(ta, j, st, tmem, sv0, b, err);
+        if (ok && next) ok = issue_s<FP8, 1>(tb, j + 1, sn, tmem, sqa, sk0, b, err);
+        ok = ok && issue_pv<1>(tb, j, st, tmem, sv0, b, err);
+        umma_commit(&b->kv_empty[st]);
+      }
+    }
+  } else {
+    setmaxnreg_inc<192>();
+    const int x = (warp - 4) >> 2;
+    const Tile t = x ? tl[1] : tl[0];
+    const int row = (warp & 3) * 32 + lane;
+    const int tr = row / a.group;
+    const bool real = tr < t.ntok;
+    const int tok = t.tok0 + tr, h = g * a.group + row % a.group;
+    const int pos = t.pos0 + tr;
+    // visible keys of this row, relative to lo
+    const int see_lo = a.window > 0 ? max(pos - a.window + 1, 0) - lo : -lo;
+    const int see_hi = real ? min(pos + 1, sq.key_end) - lo : -1;  // exclusive
+    float qmul = a.scale_log2;
+    {  // this row of Q into its tile
+      const uint4* src = reinterpret_cast<const uint4*>(a.q + (int64_t)tok * a.ld_q + (int64_t)h * kD);
+      const uint32_t dst = sbase + ChunkSmem::Q + x * kTile;
+      uint4 w[8];
+#pragma unroll
+      for (int c = 0; c < 8; ++c) w[c] = real ? src[c] : make_uint4(0, 0, 0, 0);
+      if constexpr (FP8) {
+        uint32_t m2 = 0;
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+          m2 = __vmaxu2(m2, __vmaxu2(__vmaxu2(w[c].x & 0x7fff7fffu, w[c].y & 0x7fff7fffu),
+                                     __vmaxu2(w[c].z & 0x7fff7fffu, w[c].w & 0x7fff7fffu)));
+        int e = (int)(max(m2 & 0xffffu, m2 >> 16) >> 7) - 127;  // largest magnitude in [2^e, 2^(e+1))
+        if (e > 126 || e < -126) e = 0;
+        qmul *= pow2i(e);
+        const float f = pow2i(-e);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          uint32_t* q = reinterpret_cast<uint32_t*>(&w[c]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) q[i] = h2_of(__uint_as_float(q[i] << 16) * f, __uint_as_float(q[i] & 0xffff0000u) * f);
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < 8; ++c) st4(dst + sw128(row, c), w[c].x, w[c].y, w[c].z, w[c].w);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&b->q_full);
+    }
+    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t s_addr = tmem + lane_base + kColS + x * kBK;
+    const uint32_t p_addr = tmem + lane_base + kColP + x * 64;
+    const uint32_t o_addr = tmem + lane_base + kColO + x * kD;
+    // blocks [k0, k0 + 128) with every key visible to every row of the tile
+    const int tile_lo = a.window > 0 ? max(t.pos0 + t.ntok - a.window, 0) - lo : -lo;
+    const int tile_hi = min(t.pos0 + 1, sq.key_end) - lo;
+    float m_ref = -INFINITY, l_run = 0.f;
+    int unit = 0, c = 0;
+    bool ok = true, broken_row = false;
+    for (int j = t.jlo; j < t.jhi; ++j, ++c) {
+      const int st = (j - b0) % kST;
+      // (the block's tiles are complete when S is; the wait on them is for what info holds)
+      if (!mbar_wait(&b->s_full[x], c & 1, err, &b->abort_flag) ||
+          !mbar_wait(&b->kv_full[st], ((j - b0) / kST) & 1, err, &b->abort_flag)) { ok = false; break; }
+      tc_fence_after();
+      const StageInfo* info = &b->info[st];
+      float sv[kBK];
+      {
+        uint32_t r0[32], r1[32], r2[32], r3[32];
+        tmem_ld_32x32b_x32(s_addr, r0);
+        tmem_ld_32x32b_x32(s_addr + 32, r1);
+        tmem_ld_32x32b_x32(s_addr + 64, r2);
+        tmem_ld_32x32b_x32(s_addr + 96, r3);
+        tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          sv[e] = __uint_as_float(r0[e]);
+          sv[32 + e] = __uint_as_float(r1[e]);
+          sv[64 + e] = __uint_as_float(r2[e]);
+          sv[96 + e] = __uint_as_float(r3[e]);
+        }
+      }
+      const float smul = fmaxf(FP8 ? qmul * info->kmul : qmul, 1.17549435e-38f);  // not 0: -inf * 0
+      const int new_unit = info->unit;
+      const int k0 = j * kBK;  // relative to lo
+      const uint32_t all4 = info->there[0] & info->there[1] & info->there[2] & info->there[3];
+      const bool need_mask = k0 < tile_lo || k0 + kBK > tile_hi || all4 != 0xffffffffu;
+      if (need_mask) {
+        uint32_t hit = 0;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          // bits of keys k0 + 32 w + e in [see_lo, see_hi)
+          const int f = min(max(see_lo - (k0 + 32 * w), 0), 32), e1 = min(max(see_hi - (k0 + 32 * w), 0), 32);
+          uint32_t vis = info->there[w];
+          vis &= f >= 32 ? 0u : 0xffffffffu << f;
+          vis &= e1 >= 32 ? 0xffffffffu : (1u << e1) - 1u;
+          hit |= vis & info->broken[w];
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (!((vis >> e) & 1u)) sv[32 * w + e] = -INFINITY;
+        }
+        broken_row |= hit != 0;
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&b->s_free[x]);
+      float mxp[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) mxp[u] = fmaxf(sv[u], sv[8 + u]);
+#pragma unroll
+      for (int cc = 16; cc < kBK; cc += 16) {
+#pragma unroll
+        for (int u = 0; u < 8; ++u) mxp[u] = fmax3(mxp[u], sv[cc + u], sv[cc + 8 + u]);
+      }
+      const float mraw = fmax3(fmax3(mxp[0], mxp[1], mxp[2]), fmax3(mxp[3], mxp[4], mxp[5]), fmaxf(mxp[6], mxp[7]));
+      const float cand = mraw == -INFINITY ? -INFINITY : mraw * smul - kTopLog2;
+      float alpha = 1.f;
+      bool resc = cand > m_ref + kGrowLog2;
+      if (resc) {
+        alpha = ex2a(m_ref - cand);
+        m_ref = cand;
+      }
+      const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
+      const uint64_t negm2 = pk2(-m_use, -m_use), scale2 = pk2(smul, smul);
+      uint32_t pk[kBK / 2];
+      uint64_t rs2[4] = {0ull, 0ull, 0ull, 0ull};
+#pragma unroll
+      for (int c8 = 0; c8 < kBK / 8; ++c8) {
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          float x0, x1;
+          upk2(fma2(pk2(sv[c8 * 8 + e], sv[c8 * 8 + e + 1]), scale2, negm2), x0, x1);
+          x0 = ex2a(x0);
+          x1 = ex2a(x1);
+          rs2[e / 2] = add2(rs2[e / 2], pk2(x0, x1));
+          pk[c8 * 4 + e / 2] = h2_of(x0, x1);
+        }
+      }
+      float rs0, rs1;
+      upk2(add2(add2(rs2[0], rs2[1]), add2(rs2[2], rs2[3])), rs0, rs1);
+      l_run = l_run * alpha + (rs0 + rs1);
+      if (c == 0) unit = new_unit;
+      if (new_unit != unit) {
+        alpha *= pow2i(max(unit - new_unit, -127));
+        unit = new_unit;
+        resc = true;
+      }
+      if (c > 0) {
+        if (!mbar_wait(&b->o_ready[x], (c - 1) & 1, err, &b->abort_flag)) { ok = false; break; }
+        tc_fence_after();
+        if (__any_sync(0xffffffffu, resc)) {
+#pragma unroll
+          for (int h32 = 0; h32 < kD / 32; ++h32) {
+            uint32_t r[32];
+            tmem_ld_32x32b_x32(o_addr + h32 * 32, r);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * alpha);
+            tmem_st_32x32b_x32(o_addr + h32 * 32, r);
+          }
+        }
+      }
+      {
+        uint32_t w0[32], w1[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          w0[e] = pk[e];
+          w1[e] = pk[32 + e];
+        }
+        tmem_st_32x32b_x32(p_addr, w0);
+        tmem_st_32x32b_x32(p_addr + 32, w1);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&b->p_full[x]);
+    }
+    // ---- this CTA's part of the row: o / l in fp32
+    uint32_t o0[32], o1[32];
+#pragma unroll
+    for (int e = 0; e < 32; ++e) o0[e] = o1[e] = 0u;
+    if (ok && c > 0 && mbar_wait(&b->o_ready[x], (c - 1) & 1, err, &b->abort_flag)) {
+      tc_fence_after();
+      tmem_ld_32x32b_x32(o_addr, o0);
+      tmem_ld_32x32b_x32(o_addr + 32, o1);
+      tmem_ld_wait();
+    }
+    tc_fence_before();
+    named_barrier_sync(2, 256);  // every product of this CTA is done, b->wide is final
+    if (broken_row || b->wide) l_run = __uint_as_float(0x7fc00000u);  // NaN: key by key below
+    const float sk = a.sinks != nullptr ? a.sinks[h < a.hq ? h : 0] * kLog2e : -INFINITY;
+    float inv, m_fin = m_ref;
+    if (splits == 1) {
+      m_fin = fmaxf(m_ref, sk);
+      const float mu = m_fin == -INFINITY ? 0.f : m_fin;
+      const float f = ex2a(m_ref - mu);
+      const float den = l_run * f + ex2a(sk - mu);
+      inv = den == 0.f ? 0.f : f / den;
+    } else {
+      inv = l_run == 0.f ? 0.f : 1.f / l_run;
+    }
+    inv *= pow2i(max(unit, -127));
+    bool bad = false;
+#pragma unroll
+    for (int e = 0; e < 32; ++e) {
+      const float p0 = __uint_as_float(o0[e]) * inv, p1 = __uint_as_float(o1[e]) * inv;
+      bad |= !(fabsf(p0) < INFINITY) || !(fabsf(p1) < INFINITY);
+      o0[e] = __float_as_uint(p0);
+      o1[e] = __float_as_uint(p1);
+    }
+    if (splits == 1) {
+      if (real && !bad) {
+        __nv_bfloat16* orow = a.out + (int64_t)tok * a.ld_out + (int64_t)h * kD;
+#pragma unroll
+        for (int c8 = 0; c8 < 8; ++c8) {
+          const uint32_t* s = c8 < 4 ? o0 + c8 * 8 : o1 + (c8 - 4) * 8;
+          uint4 w;
+          w.x = pack_bf16x2(__uint_as_float(s[0]), __uint_as_float(s[1]));
+          w.y = pack_bf16x2(__uint_as_float(s[2]), __uint_as_float(s[3]));
+          w.z = pack_bf16x2(__uint_as_float(s[4]), __uint_as_float(s[5]));
+          w.w = pack_bf16x2(__uint_as_float(s[6]), __uint_as_float(s[7]));
+          *reinterpret_cast<uint4*>(orow + c8 * 8) = w;
+        }
+      }
+    } else {
+      // parts lie over the K/V tiles: [256 rows][64] fp32, 16-byte chunks swizzled by the row
+      const int r = x * 128 + row;
+      const uint32_t dst = sbase + ChunkSmem::K + r * 256;
+#pragma unroll
+      for (int c16 = 0; c16 < 16; ++c16) {
+        const uint32_t* s = c16 < 8 ? o0 + c16 * 4 : o1 + (c16 - 8) * 4;
+        st4(dst + ((c16 ^ (r & 15)) << 4), s[0], s[1], s[2], s[3]);
+      }
+      b->row_m[r] = m_ref;
+      b->row_l[r] = bad ? __uint_as_float(0x7fc00000u) : l_run;
+      bad = false;
+      cg::this_cluster().sync();
+      const float* part = reinterpret_cast<const float*>(smem + ChunkSmem::K);
+      for (int rr = rank * 8 + (warp - 4); rr < 256; rr += splits * 8) {
+        const Tile& tt = rr < 128 ? tl[0] : tl[1];
+        const int rt = (rr & 127) / a.group;
+        if (rt >= tt.ntok) continue;
+        const int hh = g * a.group + (rr & 127) % a.group;
+        const float sk2 = a.sinks != nullptr ? a.sinks[hh] * kLog2e : -INFINITY;
+        float mc = -INFINITY, lc = 0.f;
+        if (lane < splits) {
+          mc = *cg::this_cluster().map_shared_rank(&b->row_m[rr], lane);
+          lc = *cg::this_cluster().map_shared_rank(&b->row_l[rr], lane);
+        }
+        float mt = fmaxf(mc, sk2);
+#pragma unroll
+        for (int y = 16; y > 0; y >>= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, y));
+        const float mu = mt == -INFINITY ? 0.f : mt;
+        const float f = lc * ex2a(mc - mu);
+        float den = f;
+#pragma unroll
+        for (int y = 16; y > 0; y >>= 1) den += __shfl_xor_sync(0xffffffffu, den, y);
+        den += ex2a(sk2 - mu);
+        float p0 = 0.f, p1 = 0.f;
+        const float* src = part + rr * 64 + (((lane >> 1) ^ (rr & 15)) << 2) + (lane & 1) * 2;
+        for (int q = 0; q < splits; ++q) {
+          const float fq = __shfl_sync(0xffffffffu, f, q);
+          const float2 v = *reinterpret_cast<const float2*>(cg::this_cluster().map_shared_rank(src, q));
+          p0 = fmaf(fq, v.x, p0);
+          p1 = fmaf(fq, v.y, p1);
+        }
+        const float iv = den == 0.f ? 0.f : 1.f / den;
+        p0 *= iv;
+        p1 *= iv;
+        if (__any_sync(0xffffffffu, !(fabsf(p0) < INFINITY && fabsf(p1) < INFINITY))) {
+          const int p = tt.pos0 + rt;
+          warp_row<FP8>(a, table, tt.tok0 + rt, hh, a.window > 0 ? max(0, p - a.window + 1) : 0, min(p + 1, sq.key_end),
+                        p0, p1);
+        }
+        reinterpret_cast<__nv_bfloat162*>(a.out + (int64_t)(tt.tok0 + rt) * a.ld_out + (int64_t)hh * kD)[lane] =
+            __floats2bfloat162_rn(p0, p1);
+      }
+    }
+    // rows to take key by key (splits == 1)
+    for (uint32_t left = __ballot_sync(0xffffffffu, bad && real); left; left &= left - 1) {
+      const int src = __ffs(left) - 1;
+      const int bt = __shfl_sync(0xffffffffu, tok, src), bh = __shfl_sync(0xffffffffu, h, src);
+      const int bp = __shfl_sync(0xffffffffu, pos, src);
+      float p0, p1;
+      warp_row<FP8>(a, table, bt, bh, a.window > 0 ? max(0, bp - a.window + 1) : 0, min(bp + 1, sq.key_end), p0, p1);
+      reinterpret_cast<__nv_bfloat162*>(a.out + (int64_t)bt * a.ld_out + (int64_t)bh * kD)[lane] =
+          __floats2bfloat162_rn(p0, p1);
+    }
+  }
+  // the other warps of a cluster meet the softmax warps' first barrier here
+  if (splits > 1) {
+    __syncwarp();
+    if (warp < 4 || warp >= 12) cg::this_cluster().sync();
+    cg::this_cluster().sync();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 13) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <bool FP8>
+static void launch_chunk_t(const Args& a, int tokens, int slots, int splits, cudaStream_t stream) {
+  auto kern = paged_chunk_kernel<FP8>;
+  constexpr int smem = ChunkSmem::INFO + 1024;
+  static bool ready[64] = {};
+  int dev;
+  AF3_CUDA_CHECK(cudaGetDevice(&dev));
+  if (!ready[dev]) {
+    AF3_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    ready[dev] = true;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(slots * splits), (unsigned)a.hkv);
+  cfg.blockDim = dim3(kChunkThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim = {(unsigned)splits, 1, 1};
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  AF3_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, a, tokens, splits, device_error_ptr()));
+}
+
+void launch_chunk(const Args& a, int64_t max_q, int64_t max_len, cudaStream_t stream) {
+  const int tokens = 128 / a.group, span = 2 * tokens;
+  // Sequence b has slots [cu[b] / span + b, cu[b + 1] / span + b + 1): at least ceil(q_b / span).
+  const int slots = a.T / span + a.B;
+  const int64_t keys = a.window > 0 ? std::min<int64_t>(max_len, a.window + std::min<int64_t>(max_q, span)) : max_len;
+  const int64_t spans = std::max<int64_t>((a.T + span - 1) / span, 1) * a.hkv;
+  int splits = 1;
+  while (splits < 8 && spans * splits * 2 <= num_sms() && keys >= 2048 * splits) splits *= 2;
+  if (a.p.ks != nullptr)
+    launch_chunk_t<true>(a, tokens, slots, splits, stream);
+  else
+    launch_chunk_t<false>(a, tokens, slots, splits, stream);
+}
+
+}  // namespace paged
+}  // namespace af3
