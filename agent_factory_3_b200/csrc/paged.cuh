@@ -54,6 +54,13 @@ __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint16_t c) {
   return r;
 }
 
+// Four e4m3 codes -> f16 pairs of the low two and of the high two.
+__device__ __forceinline__ void e4m3x4_to_f16x2(uint32_t c, uint32_t& lo, uint32_t& hi) {
+  asm("{\n.reg .b16 l, h;\nmov.b32 {l, h}, %2;\ncvt.rn.f16x2.e4m3x2 %0, l;\ncvt.rn.f16x2.e4m3x2 %1, h;\n}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(c));
+}
+
 __device__ __forceinline__ float2 f16x2_to_float2(uint32_t h) {
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }

@@ -250,8 +250,10 @@ __device__ __forceinline__ void expand16(uint32_t tile, int r, int c, const uint
   uint32_t o[8];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    o[2 * i] = hmul2(e4m3x2_to_f16x2((uint16_t)x[i]), mul);
-    o[2 * i + 1] = hmul2(e4m3x2_to_f16x2((uint16_t)(x[i] >> 16)), mul);
+    uint32_t l, h;
+    e4m3x4_to_f16x2(x[i], l, h);
+    o[2 * i] = hmul2(l, mul);
+    o[2 * i + 1] = hmul2(h, mul);
   }
   st4(tile + sw128(r, 2 * c), o[0], o[1], o[2], o[3]);
   st4(tile + sw128(r, 2 * c + 1), o[4], o[5], o[6], o[7]);

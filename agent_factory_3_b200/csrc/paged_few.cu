@@ -4,8 +4,8 @@
 //
 // Work: one cluster of S CTAs per (sequence, KV head); the CTAs take contiguous parts of the keys
 // and join over distributed shared memory, so there is one launch, no workspace, and a fixed order
-// of every sum.  In a CTA each of the four warps runs on its own: every fourth block of 32 keys,
-// copied by cp.async into the warp's ring of kStages blocks, with its own running maximum, sum
+// of every sum.  In a CTA each warp runs on its own: every fourth or eighth block of 32 keys,
+// copied by cp.async into the warp's ring, with its own running maximum, sum
 // and output, merged at the end.
 //
 // The matrix instructions (m16n8k16) run with the keys as M and the query rows as N, so 8 rows
@@ -26,6 +26,8 @@
 // behind the copies.
 #include <cooperative_groups.h>
 
+#include <type_traits>
+
 #include "host_utils.h"
 #include "paged_attention.h"
 
@@ -34,21 +36,27 @@ namespace cg = cooperative_groups;
 namespace af3 {
 namespace paged {
 
-constexpr int kWarps = 4;
-constexpr int kFewThreads = kWarps * 32;
-constexpr int kStages = 3;
-
-template <bool FP8>
+// Two shapes of CTA.  Long: 8 warps, 3 blocks in flight each.  Short (a part of at most 8 blocks:
+// short contexts, sliding windows): 4 warps with 2 blocks each, all of them on their way at once, and
+// small enough that several CTAs share an SM.
+template <bool FP8, int NT, bool LONG>
 struct FewCfg {
+  static constexpr int kWarps = LONG ? 8 : 4;
+  static constexpr int kThreads = kWarps * 32;
+  static constexpr int kStages = LONG ? 3 : 2;
   static constexpr int kRowBytes = FP8 ? 64 : 128;
   static constexpr int kStageBytes = 2 * 32 * kRowBytes;  // K then V
   static constexpr int kRingBytes = kStages * kStageBytes;
+  static constexpr int kBlocksPerSm = LONG ? (FP8 && NT <= 2 ? 2 : 1) : (NT == 1 ? 4 : NT == 2 ? 3 : 2);
   static constexpr float kTop = FP8 ? 10.f : 0.f;  // the largest p of a row is 2^kTop
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
   const int n = on ? 16 : 0;  // 0: the 16 bytes are filled with zeros and src is not read
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -128,40 +136,103 @@ __device__ __forceinline__ bool clear_nonfinite(uint32_t addr) {
 // What lane l remembers of key l of a block in flight: K and V scale bytes, and whether it exists.
 constexpr uint32_t kThere = 1u << 16;
 
-template <bool FP8>
-__device__ __forceinline__ uint32_t issue_block(const Args& a, const int* table, int g, int base, int lo, int hi,
-                                                uint32_t dst) {
-  using C = FewCfg<FP8>;
-  const int lane = threadIdx.x & 31;
-  const int j = base + lane;
-  int64_t row = 0, sc = 0;
-  uint32_t info = 0;
-  const bool there = j >= lo && j < hi && key_row(a, table, j, g, row, sc);
-  if (there) {
-    info = kThere;
-    if constexpr (FP8) info |= (uint32_t)a.p.ks[sc] | ((uint32_t)a.p.vs[sc] << 8);
-  }
-  constexpr int kChunks = C::kRowBytes / 16, kRowsPer = 32 / kChunks;
-  // the rows' offsets travel by shuffle; a missing row has offset 0 and is filled with zeros.
-  // Nothing here waits for the scale bytes.
-  const uint32_t mask = __ballot_sync(0xffffffffu, there);
-  const int c = lane % kChunks;
-#pragma unroll
-  for (int i = 0; i < 32 / kRowsPer; ++i) {
-    const int r = i * kRowsPer + lane / kChunks;
-    const int64_t off = __shfl_sync(0xffffffffu, row, r) + c * 16;
-    const bool on = (mask >> r) & 1u;
-    const uint32_t d = dst + chunk_at<FP8>(r, c);
-    cp_async16(d, a.p.k + off, on);
-    cp_async16(d + 32 * C::kRowBytes, a.p.v + off, on);
-  }
-  return info;
+// Page of key base + lane (of key base where a block lies in one page), -1 when the key is out of
+// range.  Loaded a block before it is needed.
+template <bool ONE>
+__device__ __forceinline__ int block_page(const Args& a, const int* table, int base, int lo, int hi) {
+  const int j = ONE ? base : base + (int)(threadIdx.x & 31);
+  if (!ONE && (j < lo || j >= hi)) return -1;
+  return table[a.p.page_shift >= 0 ? j >> a.p.page_shift : j / a.p.page_size];
 }
 
-template <bool FP8, int NT>
-__global__ void __launch_bounds__(kFewThreads, FP8 ? (NT == 1 ? 4 : NT == 2 ? 3 : 2) : 2) paged_few_kernel(const Args a, const int rows_per_tile,
-                                                                                const int splits) {
-  using C = FewCfg<FP8>;
+// Starts the copies of block `base` and returns what this lane has to remember of key base + lane.
+// ONE: the block lies in one page (pages of a multiple of 32 keys), so that the rows' addresses
+// differ by constants: a third of the instructions.  kb, vb: the pools at this lane's piece of row 0.
+template <class C, bool FP8, bool ONE>
+__device__ __forceinline__ uint32_t issue_block(const Args& a, const uint8_t* kb, const uint8_t* vb, const uint8_t* ksb,
+                                                const uint8_t* vsb, int page, int g, int base, int lo, int hi, uint32_t dst) {
+  const int lane = threadIdx.x & 31;
+  constexpr int kChunks = C::kRowBytes / 16, kRowsPer = 32 / kChunks;
+  const int c = lane % kChunks, r0 = lane / kChunks;
+  bool there = (uint32_t)page < (uint32_t)a.p.num_pages;
+  uint32_t pi, off, info = 0;
+  if constexpr (ONE) {
+    const bool inside = base >= lo && base + 32 <= hi;
+    if (there) {
+      split_slot(a.p, (uint32_t)base, pi, off);
+      const int64_t start = (int64_t)page * a.p.page + (int64_t)off * a.p.token;
+      const uint8_t *ks = kb + start, *vs = vb + start;
+      const int64_t step = (int64_t)kRowsPer * a.p.token;
+      if (inside) {
+#pragma unroll
+        for (int i = 0; i < 32 / kRowsPer; ++i) {
+          const uint32_t d = dst + chunk_at<FP8>(i * kRowsPer + r0, c);
+          cp_async16(d, ks);
+          cp_async16(d + 32 * C::kRowBytes, vs);
+          ks += step;
+          vs += step;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 32 / kRowsPer; ++i) {
+          const int key = base + i * kRowsPer + r0;
+          const bool on = key >= lo && key < hi;
+          const uint32_t d = dst + chunk_at<FP8>(i * kRowsPer + r0, c);
+          cp_async16(d, ks, on);
+          cp_async16(d + 32 * C::kRowBytes, vs, on);
+          ks += step;
+          vs += step;
+        }
+      }
+      there = inside || (base + lane >= lo && base + lane < hi);
+      if (there) {
+        info = kThere;
+        if constexpr (FP8) {
+          const int64_t sc = (int64_t)page * a.p.s_page + (int64_t)off * a.p.s_token;
+          info |= (uint32_t)ksb[sc] | ((uint32_t)vsb[sc] << 8);
+        }
+      }
+      return info;
+    }
+#pragma unroll
+    for (int i = 0; i < 32 / kRowsPer; ++i) {
+      const uint32_t d = dst + chunk_at<FP8>(i * kRowsPer + r0, c);
+      cp_async16(d, kb, false);
+      cp_async16(d + 32 * C::kRowBytes, vb, false);
+    }
+    return 0;
+  } else {
+    int64_t row = 0;
+    if (there) {
+      split_slot(a.p, (uint32_t)(base + lane), pi, off);
+      row = (int64_t)page * a.p.page + (int64_t)off * a.p.token + (int64_t)g * a.p.head;
+      info = kThere;
+      if constexpr (FP8) {
+        const int64_t sc = (int64_t)page * a.p.s_page + (int64_t)off * a.p.s_token + (int64_t)g * a.p.s_head;
+        info |= (uint32_t)a.p.ks[sc] | ((uint32_t)a.p.vs[sc] << 8);
+      }
+    }
+    // the rows' offsets travel by shuffle; a missing row has offset 0 and is filled with zeros.
+    // Nothing here waits for the scale bytes.
+    const uint32_t mask = __ballot_sync(0xffffffffu, there);
+#pragma unroll
+    for (int i = 0; i < 32 / kRowsPer; ++i) {
+      const int r = i * kRowsPer + r0;
+      const int64_t at = __shfl_sync(0xffffffffu, row, r) + c * 16;
+      const bool on = (mask >> r) & 1u;
+      const uint32_t d = dst + chunk_at<FP8>(r, c);
+      cp_async16(d, a.p.k + at, on);
+      cp_async16(d + 32 * C::kRowBytes, a.p.v + at, on);
+    }
+    return info;
+  }
+}
+
+template <bool FP8, int NT, bool LONG, bool ONE>
+__global__ void __launch_bounds__(FewCfg<FP8, NT, LONG>::kThreads, FewCfg<FP8, NT, LONG>::kBlocksPerSm)
+    paged_few_kernel(const Args a, const int rows_per_tile, const int splits) {
+  using C = FewCfg<FP8, NT, LONG>;
+  constexpr int kWarps = C::kWarps, kStages = C::kStages;
   constexpr int R = NT * 8;  // query rows of a tile
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float s_m[kWarps][R], s_l[kWarps][R];
@@ -177,6 +248,10 @@ __global__ void __launch_bounds__(kFewThreads, FP8 ? (NT == 1 ? 4 : NT == 2 ? 3 
   const int* table = a.table + (int64_t)b * a.ld_table;
   uint8_t* ring = smem + warp * C::kRingBytes;
   const uint32_t ring_s = (uint32_t)__cvta_generic_to_shared(ring);
+  constexpr int kChunks = C::kRowBytes / 16;
+  const int64_t piece = (int64_t)g * a.p.head + (lane / kChunks) * a.p.token + (lane % kChunks) * 16;
+  const int64_t byte = (int64_t)g * a.p.s_head + lane * a.p.s_token;
+  const uint8_t *kb0 = a.p.k + piece, *vb0 = a.p.v + piece, *ksb = a.p.ks + byte, *vsb = a.p.vs + byte;
 
   for (int tok0 = sq.t0; tok0 < sq.t1; tok0 += tokens_per_tile) {
     const int ntok = min(tokens_per_tile, sq.t1 - tok0);
@@ -249,11 +324,17 @@ __global__ void __launch_bounds__(kFewThreads, FP8 ? (NT == 1 ? 4 : NT == 2 ? 3 
 
     uint32_t info[kStages];
     const int first = my0 + warp;
+    int ahead_page = -1;  // pages of the next block to copy
+    if (first < my1) ahead_page = block_page<ONE>(a, table, first * 32, lo, hi);
 #pragma unroll
     for (int s = 0; s < kStages - 1; ++s) {
       info[s] = 0;
-      if (first + s * kWarps < my1)
-        info[s] = issue_block<FP8>(a, table, g, (first + s * kWarps) * 32, lo, hi, ring_s + s * C::kStageBytes);
+      const int cur = first + s * kWarps;
+      if (cur < my1) {
+        const int page = ahead_page;
+        if (cur + kWarps < my1) ahead_page = block_page<ONE>(a, table, (cur + kWarps) * 32, lo, hi);
+        info[s] = issue_block<C, FP8, ONE>(a, kb0, vb0, ksb, vsb, page, g, cur * 32, lo, hi, ring_s + s * C::kStageBytes);
+      }
       cp_async_commit();
     }
     for (int blk = first; blk < my1; blk += kStages * kWarps) {
@@ -266,7 +347,12 @@ __global__ void __launch_bounds__(kFewThreads, FP8 ? (NT == 1 ? 4 : NT == 2 ? 3 
           const int slot = (s + ahead) % kStages;
           const int nxt = cur + ahead * kWarps;
           __syncwarp();  // every lane has read the block that this slot held
-          if (nxt < my1) info[slot] = issue_block<FP8>(a, table, g, nxt * 32, lo, hi, ring_s + slot * C::kStageBytes);
+          if (nxt < my1) {
+            const int page = ahead_page;
+            if (nxt + kWarps < my1) ahead_page = block_page<ONE>(a, table, (nxt + kWarps) * 32, lo, hi);
+            info[slot] = issue_block<C, FP8, ONE>(a, kb0, vb0, ksb, vsb, page, g, nxt * 32, lo, hi,
+                                                       ring_s + slot * C::kStageBytes);
+          }
           cp_async_commit();
         }
         cp_async_wait<kStages - 1>();
@@ -299,8 +385,9 @@ __global__ void __launch_bounds__(kFewThreads, FP8 ? (NT == 1 ? 4 : NT == 2 ? 3 
             const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks) {
-              const uint32_t a0 = e4m3x2_to_f16x2((uint16_t)xw[ks]), a2 = e4m3x2_to_f16x2((uint16_t)(xw[ks] >> 16));
-              const uint32_t a1 = e4m3x2_to_f16x2((uint16_t)yw[ks]), a3 = e4m3x2_to_f16x2((uint16_t)(yw[ks] >> 16));
+              uint32_t a0, a1, a2, a3;
+              e4m3x4_to_f16x2(xw[ks], a0, a2);
+              e4m3x4_to_f16x2(yw[ks], a1, a3);
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt)
                 mma16816<true>(sc[mt][nt], a0, a1, a2, a3, qf[nt][2 * ks], qf[nt][2 * ks + 1]);
@@ -337,8 +424,8 @@ __global__ void __launch_bounds__(kFewThreads, FP8 ? (NT == 1 ? 4 : NT == 2 ? 3 
           const uint32_t inf = __shfl_sync(0xffffffffu, info[s], grp + 8 * k);
           float kmul = 1.f;
           if constexpr (FP8) {
-            kmul = pow2i((int)(inf & 255u) - 127);
-            vmul[k] = pow2i(max((int)((inf >> 8) & 255u) - vmax, -127));
+            kmul = __uint_as_float((inf & 255u) << 23);  // byte 0: values below 2^-118 count as 0
+            vmul[k] = __uint_as_float((uint32_t)max((int)((inf >> 8) & 255u) - vmax + 127, 0) << 23);
           }
           const int key = base + grp + 8 * k;
 #pragma unroll
@@ -438,8 +525,9 @@ __global__ void __launch_bounds__(kFewThreads, FP8 ? (NT == 1 ? 4 : NT == 2 ? 3 
               const uint32_t sel = (i & 1) ? 0x7362u : 0x5140u;
               const uint32_t xy = __byte_perm(i < 2 ? x.x : x.y, i < 2 ? y.x : y.y, sel);
               const uint32_t zu = __byte_perm(i < 2 ? z.x : z.y, i < 2 ? u.x : u.y, sel);
-              const uint32_t a0 = e4m3x2_to_f16x2((uint16_t)xy), a1 = e4m3x2_to_f16x2((uint16_t)(xy >> 16));
-              const uint32_t a2 = e4m3x2_to_f16x2((uint16_t)zu), a3 = e4m3x2_to_f16x2((uint16_t)(zu >> 16));
+              uint32_t a0, a1, a2, a3;
+              e4m3x4_to_f16x2(xy, a0, a1);
+              e4m3x4_to_f16x2(zu, a2, a3);
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) mma16816<true>(o[nt][i], a0, a1, a2, a3, pb[mt][nt][0], pb[mt][nt][1]);
             }
@@ -567,55 +655,63 @@ __global__ void __launch_bounds__(kFewThreads, FP8 ? (NT == 1 ? 4 : NT == 2 ? 3 
   }
 }
 
-template <bool FP8, int NT>
+template <bool FP8, int NT, bool LONG, bool ONE>
 static void launch_few_nt(const Args& a, int rows_per_tile, int splits, cudaStream_t stream) {
-  using C = FewCfg<FP8>;
-  constexpr int smem = kWarps * C::kRingBytes + NT * 8 * kD * 4;
+  using C = FewCfg<FP8, NT, LONG>;
+  constexpr int smem = C::kWarps * C::kRingBytes + NT * 8 * kD * 4;
   static_assert(NT * 8 * kD * 4 <= C::kRingBytes, "a warp's part has to fit its ring");
-  auto kern = paged_few_kernel<FP8, NT>;
+  auto kern = paged_few_kernel<FP8, NT, LONG, ONE>;
   static bool ready[64] = {};
   int dev;
   AF3_CUDA_CHECK(cudaGetDevice(&dev));
   if (!ready[dev]) {
     AF3_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    AF3_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     ready[dev] = true;
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)splits, (unsigned)a.hkv, (unsigned)a.B);
-  cfg.blockDim = dim3(kFewThreads);
+  cfg.blockDim = dim3(C::kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim = {(unsigned)splits, 1, 1};
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = splits > 1 ? 1 : 0;
   AF3_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, a, rows_per_tile, splits));
 }
 
-template <bool FP8>
+template <bool FP8, bool LONG, bool ONE>
 static void launch_few_t(const Args& a, int max_q, int splits, cudaStream_t stream) {
   const int want = std::max(std::min(max_q, kFewRows / a.group), 1) * a.group;  // rows of a tile
   if (want <= 8)
-    launch_few_nt<FP8, 1>(a, want, splits, stream);
+    launch_few_nt<FP8, 1, LONG, ONE>(a, want, splits, stream);
   else if (want <= 16)
-    launch_few_nt<FP8, 2>(a, want, splits, stream);
+    launch_few_nt<FP8, 2, LONG, ONE>(a, want, splits, stream);
   else
-    launch_few_nt<FP8, 4>(a, want, splits, stream);
+    launch_few_nt<FP8, 4, LONG, ONE>(a, want, splits, stream);
 }
 
 void launch_few(const Args& a, int64_t max_q, int64_t max_len, cudaStream_t stream) {
-  // Keys are split until the machine has about four CTAs an SM to choose from, as long as a part
-  // has 256 keys (two blocks a warp); 16 CTAs is the largest cluster.
   const int64_t keys = a.window > 0 ? std::min<int64_t>(max_len, a.window + max_q) : max_len;
-  const int64_t items = (int64_t)a.B * a.hkv, enough = 4 * (int64_t)num_sms();
+  const int64_t items = (int64_t)a.B * a.hkv;
+  // The keys are split until there are several CTAs for each SM to even out ragged lengths, as long
+  // as a part has 512 keys (two blocks a warp).  8 CTAs is the largest portable cluster.
   int splits = 1;
-  while (splits < 16 && items * splits < enough && keys >= 512 * splits) splits *= 2;
-  if (a.p.ks != nullptr)
-    launch_few_t<true>(a, (int)std::min<int64_t>(max_q, kFewRows), splits, stream);
-  else
-    launch_few_t<false>(a, (int)std::min<int64_t>(max_q, kFewRows), splits, stream);
+  const int64_t enough = 4 * (int64_t)num_sms();
+  while (splits < 8 && items * splits < enough && keys >= 512 * splits) splits *= 2;
+  if (getenv("DBG_SPLIT")) splits = atoi(getenv("DBG_SPLIT"));
+  const int q = (int)std::min<int64_t>(max_q, kFewRows);
+  const bool is_long = keys > 9 * 32 * splits;  // more than 8 blocks wherever the first one begins
+  const bool one = (a.p.page_size & 31) == 0;
+  auto go = [&](auto fp8, auto lng, auto on) {
+    launch_few_t<decltype(fp8)::value, decltype(lng)::value, decltype(on)::value>(a, q, splits, stream);
+  };
+  using T = std::true_type;
+  using F = std::false_type;
+  auto pick2 = [&](auto fp8, auto lng) { one ? go(fp8, lng, T{}) : go(fp8, lng, F{}); };
+  auto pick = [&](auto fp8) { is_long ? pick2(fp8, T{}) : pick2(fp8, F{}); };
+  a.p.ks != nullptr ? pick(T{}) : pick(F{});
 }
 
 }  // namespace paged
