@@ -65,5 +65,14 @@ __device__ __forceinline__ float2 f16x2_to_float2(uint32_t h) {
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
+// A byte, 0 where not on, in one predicated load: no branch for the result to be waited for in.
+__device__ __forceinline__ uint32_t load_byte(const uint8_t* p, bool on) {
+  uint32_t r;
+  asm volatile("{\n.reg .pred q;\nsetp.ne.b32 q, %2, 0;\nmov.b32 %0, 0;\n@q ld.global.nc.u8 %0, [%1];\n}"
+               : "=r"(r)
+               : "l"(p), "r"((int)on));
+  return r;
+}
+
 }  // namespace paged
 }  // namespace af3

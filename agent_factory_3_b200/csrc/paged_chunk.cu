@@ -206,12 +206,25 @@ struct Ahead {
   int64_t scale;  // offset of the lane's scale bytes
 };
 
+// Page of key j, -1 when it is out of range; loaded a block before it is needed.
+__device__ __forceinline__ int page_of(const Args& a, const int* table, int j, int hi) {
+  int page = -1;
+  const int pi = a.p.page_shift >= 0 ? j >> a.p.page_shift : j / a.p.page_size;
+  if (j < hi) page = table[pi];
+  return page;
+}
+
 template <bool FP8>
-__device__ __forceinline__ Ahead load_block(const Args& a, const int* table, int g, int k0, int lo, int hi, int w, int lane,
-                                            uint32_t raw, uint32_t kdst) {
-  const int j = k0 + 32 * w + lane;
+__device__ __forceinline__ Ahead load_block(const Args& a, int page, int g, int k0, int w, int lane, uint32_t raw,
+                                            uint32_t kdst) {
+  const bool on = (uint32_t)page < (uint32_t)a.p.num_pages;
   int64_t row = 0, sc = 0;
-  const bool on = j >= lo && j < hi && key_row(a, table, j, g, row, sc);
+  if (on) {
+    uint32_t pi, off;
+    split_slot(a.p, (uint32_t)(k0 + 32 * w + lane), pi, off);
+    row = (int64_t)page * a.p.page + (int64_t)off * a.p.token + (int64_t)g * a.p.head;
+    sc = (int64_t)page * a.p.s_page + (int64_t)off * a.p.s_token + (int64_t)g * a.p.s_head;
+  }
   Ahead h;
   h.there = __ballot_sync(0xffffffffu, on);
   h.scale = sc;
@@ -324,17 +337,25 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
     uint32_t top = 0;  // V: largest e8m0 byte (e4m3) or biased exponent (bf16) so far
     bool dead = false;
     Ahead ah[kRaw];
-    uint32_t scale_bytes = 0;  // of the next block to expand: K | V << 8
+    // scale bytes of the next block to expand, as loaded: combining them here would wait for them
+    uint32_t next_k = 0, next_v = 0;
     auto fetch_scales = [&](const Ahead& h) {
-      scale_bytes = 0;
-      if (FP8 && ((h.there >> lane) & 1u)) scale_bytes = (uint32_t)a.p.ks[h.scale] | ((uint32_t)a.p.vs[h.scale] << 8);
+      if constexpr (FP8) {
+        next_k = load_byte(a.p.ks + h.scale, (h.there >> lane) & 1u);
+        next_v = load_byte(a.p.vs + h.scale, (h.there >> lane) & 1u);
+      }
     };
+    const int lane_key = lo + 32 * w + lane;
+    int first_pages[kRaw];
+#pragma unroll
+    for (int i = 0; i < kRaw; ++i) first_pages[i] = b0 + i < b1 ? page_of(a, table, lane_key + (b0 + i) * kBK, hi) : -1;
+    int next_page = b0 + kRaw < b1 ? page_of(a, table, lane_key + (b0 + kRaw) * kBK, hi) : -1;
 #pragma unroll
     for (int i = 0; i < kRaw; ++i) {
       ah[i].there = 0;
       ah[i].scale = 0;
       if (b0 + i < b1)
-        ah[i] = load_block<FP8>(a, table, g, lo + (b0 + i) * kBK, lo, hi, w, lane, sbase + ChunkSmem::RAW + i * kTile,
+        ah[i] = load_block<FP8>(a, first_pages[i], g, lo + (b0 + i) * kBK, w, lane, sbase + ChunkSmem::RAW + i * kTile,
                                 sbase + ChunkSmem::K + i * kTile);
       asm volatile("cp.async.commit_group;" ::: "memory");
     }
@@ -342,6 +363,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
     int raw_slot = 0;
     for (int j = b0; j < b1; ++j) {
       const int n = j - b0, st = n % kST;
+      const uint32_t scale_bytes = next_k | (next_v << 8);
       const uint32_t raw = sbase + ChunkSmem::RAW + raw_slot * kTile;
       const uint32_t own = raw + (32 * w + lane) * 16;
       const uint32_t ktile = sbase + ChunkSmem::K + st * kTile, vtile = sbase + ChunkSmem::V + st * kTile;
@@ -479,8 +501,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
         if (!FP8 && !dead && n + kRaw >= kST &&   // K goes straight into its tile
             !mbar_wait(&b->kv_empty[ns], (((n + kRaw) / kST) & 1) ^ 1, err, &b->abort_flag))
           dead = true;
-        ah[kRaw - 1] = load_block<FP8>(a, table, g, lo + (j + kRaw) * kBK, lo, hi, w, lane, raw,
-                                       sbase + ChunkSmem::K + ns * kTile);
+        const int page = next_page;
+        if (j + kRaw + 1 < b1) next_page = page_of(a, table, lane_key + (j + kRaw + 1) * kBK, hi);
+        ah[kRaw - 1] = load_block<FP8>(a, page, g, lo + (j + kRaw) * kBK, w, lane, raw, sbase + ChunkSmem::K + ns * kTile);
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
       fetch_scales(ah[0]);

@@ -41,13 +41,16 @@ namespace paged {
 // small enough that several CTAs share an SM.
 template <bool FP8, int NT, bool LONG>
 struct FewCfg {
-  static constexpr int kWarps = LONG ? 8 : 4;
+  static constexpr int kSub = LONG && FP8 && NT <= 2 ? 2 : 1;  // a block is kSub x 32 keys
+  static constexpr int kKeys = 32 * kSub;
+  static constexpr int kWarps = LONG && kSub == 1 ? 8 : 4;
   static constexpr int kThreads = kWarps * 32;
-  static constexpr int kStages = LONG ? 3 : 2;
+  static constexpr int kStages = LONG && kSub == 1 ? 3 : 2;
   static constexpr int kRowBytes = FP8 ? 64 : 128;
-  static constexpr int kStageBytes = 2 * 32 * kRowBytes;  // K then V
+  static constexpr int kSubBytes = 2 * 32 * kRowBytes;  // K then V of 32 keys
+  static constexpr int kStageBytes = kSub * kSubBytes;
   static constexpr int kRingBytes = kStages * kStageBytes;
-  static constexpr int kBlocksPerSm = LONG ? (FP8 && NT <= 2 ? 2 : 1) : (NT == 1 ? 4 : NT == 2 ? 3 : 2);
+  static constexpr int kBlocksPerSm = LONG ? (kSub == 2 ? 3 : 1) : (NT == 1 ? 4 : NT == 2 ? 3 : 2);
   static constexpr float kTop = FP8 ? 10.f : 0.f;  // the largest p of a row is 2^kTop
 };
 
@@ -133,8 +136,11 @@ __device__ __forceinline__ bool clear_nonfinite(uint32_t addr) {
   return bad;
 }
 
-// What lane l remembers of key l of a block in flight: K and V scale bytes, and whether it exists.
-constexpr uint32_t kThere = 1u << 16;
+// What is remembered of 32 keys on their way: the ones that exist, and lane l's scale bytes of key l.
+// The bytes stay as loaded until the block is used; combining them at once would wait for them.
+struct Keys {
+  uint32_t there, k, v;
+};
 
 // Page of key base + lane (of key base where a block lies in one page), -1 when the key is out of
 // range.  Loaded a block before it is needed.
@@ -145,17 +151,18 @@ __device__ __forceinline__ int block_page(const Args& a, const int* table, int b
   return table[a.p.page_shift >= 0 ? j >> a.p.page_shift : j / a.p.page_size];
 }
 
-// Starts the copies of block `base` and returns what this lane has to remember of key base + lane.
+// Starts the copies of keys base .. base + 31.
 // ONE: the block lies in one page (pages of a multiple of 32 keys), so that the rows' addresses
 // differ by constants: a third of the instructions.  kb, vb: the pools at this lane's piece of row 0.
 template <class C, bool FP8, bool ONE>
-__device__ __forceinline__ uint32_t issue_block(const Args& a, const uint8_t* kb, const uint8_t* vb, const uint8_t* ksb,
+__device__ __forceinline__ Keys issue_block(const Args& a, const uint8_t* kb, const uint8_t* vb, const uint8_t* ksb,
                                                 const uint8_t* vsb, int page, int g, int base, int lo, int hi, uint32_t dst) {
   const int lane = threadIdx.x & 31;
   constexpr int kChunks = C::kRowBytes / 16, kRowsPer = 32 / kChunks;
   const int c = lane % kChunks, r0 = lane / kChunks;
   bool there = (uint32_t)page < (uint32_t)a.p.num_pages;
-  uint32_t pi, off, info = 0;
+  uint32_t pi, off;
+  Keys info{0, 0, 0};
   if constexpr (ONE) {
     const bool inside = base >= lo && base + 32 <= hi;
     if (there) {
@@ -184,13 +191,12 @@ __device__ __forceinline__ uint32_t issue_block(const Args& a, const uint8_t* kb
           vs += step;
         }
       }
-      there = inside || (base + lane >= lo && base + lane < hi);
-      if (there) {
-        info = kThere;
-        if constexpr (FP8) {
-          const int64_t sc = (int64_t)page * a.p.s_page + (int64_t)off * a.p.s_token;
-          info |= (uint32_t)ksb[sc] | ((uint32_t)vsb[sc] << 8);
-        }
+      const bool mine = inside || (base + lane >= lo && base + lane < hi);
+      info.there = __ballot_sync(0xffffffffu, mine);
+      if constexpr (FP8) {
+        const int64_t sc = (int64_t)page * a.p.s_page + (int64_t)off * a.p.s_token;
+        info.k = load_byte(ksb + sc, mine);
+        info.v = load_byte(vsb + sc, mine);
       }
       return info;
     }
@@ -200,21 +206,21 @@ __device__ __forceinline__ uint32_t issue_block(const Args& a, const uint8_t* kb
       cp_async16(d, kb, false);
       cp_async16(d + 32 * C::kRowBytes, vb, false);
     }
-    return 0;
+    return info;
   } else {
-    int64_t row = 0;
+    int64_t row = 0, sc = 0;
     if (there) {
       split_slot(a.p, (uint32_t)(base + lane), pi, off);
       row = (int64_t)page * a.p.page + (int64_t)off * a.p.token + (int64_t)g * a.p.head;
-      info = kThere;
-      if constexpr (FP8) {
-        const int64_t sc = (int64_t)page * a.p.s_page + (int64_t)off * a.p.s_token + (int64_t)g * a.p.s_head;
-        info |= (uint32_t)a.p.ks[sc] | ((uint32_t)a.p.vs[sc] << 8);
-      }
+      sc = (int64_t)page * a.p.s_page + (int64_t)off * a.p.s_token + (int64_t)g * a.p.s_head;
     }
-    // the rows' offsets travel by shuffle; a missing row has offset 0 and is filled with zeros.
-    // Nothing here waits for the scale bytes.
+    if constexpr (FP8) {
+      info.k = load_byte(a.p.ks + sc, there);
+      info.v = load_byte(a.p.vs + sc, there);
+    }
+    // the rows' offsets travel by shuffle; a missing row has offset 0 and is filled with zeros
     const uint32_t mask = __ballot_sync(0xffffffffu, there);
+    info.there = mask;
 #pragma unroll
     for (int i = 0; i < 32 / kRowsPer; ++i) {
       const int r = i * kRowsPer + r0;
@@ -261,9 +267,38 @@ __global__ void __launch_bounds__(FewCfg<FP8, NT, LONG>::kThreads, FewCfg<FP8, N
     // keys that any row of the tile may see
     const int lo = a.window > 0 ? max(0, pos0 - a.window + 1) : 0;
     const int hi = min(pos0 + ntok, sq.key_end);
-    const int blk0 = lo >> 5, blk1 = max((hi + 31) >> 5, blk0);
+    const int blk0 = lo / C::kKeys, blk1 = max((hi + C::kKeys - 1) / C::kKeys, blk0);
     const int per = (blk1 - blk0 + splits - 1) / splits;
     const int my0 = min(blk0 + rank * per, blk1), my1 = min(my0 + per, blk1);
+
+    // ---- the first copies, before anything waits for the query rows
+    Keys info[kStages][C::kSub];
+    const int first = my0 + warp;
+    int ahead_page[C::kSub];  // pages of the next block to copy
+    auto load_pages = [&](int blk) {
+#pragma unroll
+      for (int u = 0; u < C::kSub; ++u)
+        if (C::kSub == 1 || (blk * C::kSub + u) * 32 < hi)
+          ahead_page[u] = block_page<ONE>(a, table, (blk * C::kSub + u) * 32, lo, hi);
+        else
+          ahead_page[u] = -1;
+    };
+    auto copy_block = [&](int blk, Keys (&inf)[C::kSub], uint32_t dst) {
+      int page[C::kSub];
+#pragma unroll
+      for (int u = 0; u < C::kSub; ++u) page[u] = ahead_page[u];
+      if (blk + kWarps < my1) load_pages(blk + kWarps);
+#pragma unroll
+      for (int u = 0; u < C::kSub; ++u)
+        inf[u] = issue_block<C, FP8, ONE>(a, kb0, vb0, ksb, vsb, page[u], g, (blk * C::kSub + u) * 32, lo, hi,
+                                          dst + u * C::kSubBytes);
+    };
+    if (first < my1) load_pages(first);
+#pragma unroll
+    for (int s = 0; s < kStages - 1; ++s) {
+      if (first + s * kWarps < my1) copy_block(first + s * kWarps, info[s], ring_s + s * C::kStageBytes);
+      cp_async_commit();
+    }
 
     // ---- query rows: thread (grp, tig) holds dims [16 tig, 16 tig + 16) of rows nt * 8 + grp
     uint32_t qf[NT][8];
@@ -322,21 +357,6 @@ __global__ void __launch_bounds__(FewCfg<FP8, NT, LONG>::kThreads, FewCfg<FP8, N
       for (int i = 0; i < 4; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
     }
 
-    uint32_t info[kStages];
-    const int first = my0 + warp;
-    int ahead_page = -1;  // pages of the next block to copy
-    if (first < my1) ahead_page = block_page<ONE>(a, table, first * 32, lo, hi);
-#pragma unroll
-    for (int s = 0; s < kStages - 1; ++s) {
-      info[s] = 0;
-      const int cur = first + s * kWarps;
-      if (cur < my1) {
-        const int page = ahead_page;
-        if (cur + kWarps < my1) ahead_page = block_page<ONE>(a, table, (cur + kWarps) * 32, lo, hi);
-        info[s] = issue_block<C, FP8, ONE>(a, kb0, vb0, ksb, vsb, page, g, cur * 32, lo, hi, ring_s + s * C::kStageBytes);
-      }
-      cp_async_commit();
-    }
     for (int blk = first; blk < my1; blk += kStages * kWarps) {
 #pragma unroll
       for (int s = 0; s < kStages; ++s) {
@@ -347,39 +367,45 @@ __global__ void __launch_bounds__(FewCfg<FP8, NT, LONG>::kThreads, FewCfg<FP8, N
           const int slot = (s + ahead) % kStages;
           const int nxt = cur + ahead * kWarps;
           __syncwarp();  // every lane has read the block that this slot held
-          if (nxt < my1) {
-            const int page = ahead_page;
-            if (nxt + kWarps < my1) ahead_page = block_page<ONE>(a, table, (nxt + kWarps) * 32, lo, hi);
-            info[slot] = issue_block<C, FP8, ONE>(a, kb0, vb0, ksb, vsb, page, g, nxt * 32, lo, hi,
-                                                       ring_s + slot * C::kStageBytes);
-          }
+          if (nxt < my1) copy_block(nxt, info[slot], ring_s + slot * C::kStageBytes);
           cp_async_commit();
         }
         cp_async_wait<kStages - 1>();
         __syncwarp();
-        const uint32_t kb = ring_s + s * C::kStageBytes, vb = kb + 32 * C::kRowBytes;
-        const int base = cur * 32;
+        const uint32_t kv = ring_s + s * C::kStageBytes;
+        const int base = cur * C::kKeys;
 
+        uint32_t there[C::kSub], broken[C::kSub];  // a bit for each key
+        bool full = base >= full_lo && base + C::kKeys <= full_hi;
+#pragma unroll
+        for (int u = 0; u < C::kSub; ++u) {
+          there[u] = info[s][u].there;
+          full &= there[u] == 0xffffffffu;
+          broken[u] = 0;
+        }
         // A value that is not finite would reach every row through 0 * inf.  Where rows differ in
         // what they see, such values are taken out of the block (which leaves the rows that do not
         // see them as they are), and the rows that see them are taken again at the end.
-        const bool full = base >= full_lo && base + 32 <= full_hi && __all_sync(0xffffffffu, info[s] & kThere);
-        uint32_t broken = 0;  // keys
         if (several && !full) {
-          bool bad = false;
+#pragma unroll
+          for (int u = 0; u < C::kSub; ++u) {
+            bool bad = false;
 #pragma unroll 1
-          for (int c = 0; c < C::kRowBytes / 16; ++c) bad |= clear_nonfinite<FP8>(vb + chunk_at<FP8>(lane, c));
-          broken = __ballot_sync(0xffffffffu, bad);
+            for (int c = 0; c < C::kRowBytes / 16; ++c)
+              bad |= clear_nonfinite<FP8>(kv + u * C::kSubBytes + 32 * C::kRowBytes + chunk_at<FP8>(lane, c));
+            broken[u] = __ballot_sync(0xffffffffu, bad);
+          }
           __syncwarp();
         }
 
         // ---- S^T, keys base + 16 mt + {grp, grp + 8}
-        float sc[2][NT][4];
+        float sc[2 * C::kSub][NT][4];
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt) {
+        for (int mt = 0; mt < 2 * C::kSub; ++mt) {
+          const uint32_t kb = kv + (mt >> 1) * C::kSubBytes;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) sc[mt][nt][0] = sc[mt][nt][1] = sc[mt][nt][2] = sc[mt][nt][3] = 0.f;
-          const int r0 = mt * 16 + grp, r1 = r0 + 8;
+          const int r0 = (mt & 1) * 16 + grp, r1 = r0 + 8;
           if constexpr (FP8) {
             const uint4 x = lds128(kb + chunk_at<true>(r0, tig)), y = lds128(kb + chunk_at<true>(r1, tig));
             const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
@@ -405,39 +431,56 @@ __global__ void __launch_bounds__(FewCfg<FP8, NT, LONG>::kThreads, FewCfg<FP8, N
             }
           }
         }
-        // ---- scales of this thread's four keys, masks
-        float vmul[4];
+        // ---- scales of this thread's keys (computed by the key's lane), masks
+        float kmul[4 * C::kSub], vmul[4 * C::kSub];
         bool grew = false;
         float shrink = 1.f;
         if constexpr (FP8) {
-          const int mine = (info[s] & kThere) && !((broken >> lane) & 1u) ? (int)((info[s] >> 8) & 255u) : 0;
-          const int top = (int)__reduce_max_sync(0xffffffffu, (unsigned)mine);
-          vmin = min(vmin, mine > 0 ? mine : 255);
+          int mine[C::kSub];
+          int most = 0;
+#pragma unroll
+          for (int u = 0; u < C::kSub; ++u) {
+            mine[u] = ((broken[u] >> lane) & 1u) ? 0 : (int)info[s][u].v;  // absent: 0
+            vmin = min(vmin, mine[u] > 0 ? mine[u] : 255);
+            most = max(most, mine[u]);
+          }
+          const int top = (int)__reduce_max_sync(0xffffffffu, (unsigned)most);
           grew = top > vmax;
           if (grew) {
             shrink = pow2i(max(vmax - top, -127));
             vmax = top;
           }
+#pragma unroll
+          for (int u = 0; u < C::kSub; ++u) {
+            const float kf = __uint_as_float(info[s][u].k << 23);  // byte 0: below 2^-118, counts as 0
+            const float vf = __uint_as_float((uint32_t)max(mine[u] - vmax + 127, 0) << 23);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              kmul[4 * u + k] = __shfl_sync(0xffffffffu, kf, grp + 8 * k);
+              vmul[4 * u + k] = __shfl_sync(0xffffffffu, vf, grp + 8 * k);
+            }
+          }
         }
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {  // keys grp + 8 k: mt = k / 2, accumulator half k % 2
-          const uint32_t inf = __shfl_sync(0xffffffffu, info[s], grp + 8 * k);
-          float kmul = 1.f;
-          if constexpr (FP8) {
-            kmul = __uint_as_float((inf & 255u) << 23);  // byte 0: values below 2^-118 count as 0
-            vmul[k] = __uint_as_float((uint32_t)max((int)((inf >> 8) & 255u) - vmax + 127, 0) << 23);
-          }
-          const int key = base + grp + 8 * k;
+        for (int k = 0; k < 4 * C::kSub; ++k) {  // keys grp + 8 k: mt = k / 2, accumulator half k % 2
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              float& x = sc[k >> 1][nt][2 * (k & 1) + c];
-              x *= FP8 ? smul[nt][c] * kmul : smul[nt][c];
-              if (!full) {
-                if (!((inf & kThere) && key >= rlo[nt][c] && key <= rhi[nt][c]))
-                  x = -INFINITY;
-                else if ((broken >> (grp + 8 * k)) & 1u)
+            for (int c = 0; c < 2; ++c) sc[k >> 1][nt][2 * (k & 1) + c] *= FP8 ? smul[nt][c] * kmul[k] : smul[nt][c];
+          }
+        }
+        if (!full) {
+#pragma unroll
+          for (int k = 0; k < 4 * C::kSub; ++k) {
+            const int bit = grp + 8 * (k & 3), key = base + grp + 8 * k;
+            const bool on = (there[k >> 2] >> bit) & 1u, bad = (broken[k >> 2] >> bit) & 1u;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                if (!(on && key >= rlo[nt][c] && key <= rhi[nt][c]))
+                  sc[k >> 1][nt][2 * (k & 1) + c] = -INFINITY;
+                else if (bad)
                   l[nt][c] = __uint_as_float(0x7fc00000u);
               }
             }
@@ -450,8 +493,10 @@ __global__ void __launch_bounds__(FewCfg<FP8, NT, LONG>::kThreads, FewCfg<FP8, N
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            mx[nt][c] = fmaxf(fmaxf(sc[0][nt][c], sc[0][nt][2 + c]), fmaxf(sc[1][nt][c], sc[1][nt][2 + c]));
-            mx[nt][c] -= C::kTop;
+            float x = fmaxf(sc[0][nt][c], sc[0][nt][2 + c]);
+#pragma unroll
+            for (int mt = 1; mt < 2 * C::kSub; ++mt) x = fmaxf(x, fmaxf(sc[mt][nt][c], sc[mt][nt][2 + c]));
+            mx[nt][c] = x - C::kTop;
             need |= mx[nt][c] > m[nt][c];
           }
         }
@@ -487,12 +532,12 @@ __global__ void __launch_bounds__(FewCfg<FP8, NT, LONG>::kThreads, FewCfg<FP8, N
             }
         }
         // ---- P^T as B fragments
-        uint32_t pb[2][NT][2], pl[2][NT][2];  // pl: what pb's bf16 leaves out
+        uint32_t pb[2 * C::kSub][NT][2], pl[2 * C::kSub][NT][2];  // pl: what pb's bf16 leaves out
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           const float mu0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0], mu1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
+          for (int k = 0; k < 4 * C::kSub; ++k) {
             float p0 = ex2a(sc[k >> 1][nt][2 * (k & 1)] - mu0);
             float p1 = ex2a(sc[k >> 1][nt][2 * (k & 1) + 1] - mu1);
             l[nt][0] += p0;
@@ -510,8 +555,9 @@ __global__ void __launch_bounds__(FewCfg<FP8, NT, LONG>::kThreads, FewCfg<FP8, N
         }
         // ---- O^T += V^T P^T
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt) {
-          const int r = mt * 16 + 2 * tig;
+        for (int mt = 0; mt < 2 * C::kSub; ++mt) {
+          const uint32_t vb = kv + (mt >> 1) * C::kSubBytes + 32 * C::kRowBytes;
+          const int r = (mt & 1) * 16 + 2 * tig;
           if constexpr (FP8) {
             // dims [8 grp, 8 grp + 8): half of chunk grp / 2
             const uint32_t in = (uint32_t)(grp & 1) * 8;
@@ -655,57 +701,81 @@ __global__ void __launch_bounds__(FewCfg<FP8, NT, LONG>::kThreads, FewCfg<FP8, N
   }
 }
 
+// How many clusters of `splits` CTAs the device holds at once.  Clusters lie within one GPC, so this
+// is less than the number of CTAs that fit divided by the size (16 clusters of 6 fit, not of 7).
+template <class K>
+static int clusters_at_once(K kern, const cudaLaunchConfig_t& cfg) {
+  int n = 0;
+  AF3_CUDA_CHECK(cudaOccupancyMaxActiveClusters(&n, kern, &cfg));
+  return std::max(n, 1);
+}
+
 template <bool FP8, int NT, bool LONG, bool ONE>
-static void launch_few_nt(const Args& a, int rows_per_tile, int splits, cudaStream_t stream) {
+static void launch_few_nt(const Args& a, int rows_per_tile, int64_t keys, cudaStream_t stream) {
   using C = FewCfg<FP8, NT, LONG>;
   constexpr int smem = C::kWarps * C::kRingBytes + NT * 8 * kD * 4;
   static_assert(NT * 8 * kD * 4 <= C::kRingBytes, "a warp's part has to fit its ring");
   auto kern = paged_few_kernel<FP8, NT, LONG, ONE>;
-  static bool ready[64] = {};
+  constexpr int kMaxSplits = 8;  // the largest portable cluster
+  static int at_once[64][kMaxSplits + 1] = {};
   int dev;
   AF3_CUDA_CHECK(cudaGetDevice(&dev));
-  if (!ready[dev]) {
-    AF3_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    ready[dev] = true;
-  }
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)splits, (unsigned)a.hkv, (unsigned)a.B);
   cfg.blockDim = dim3(C::kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim = {(unsigned)splits, 1, 1};
   cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (at_once[dev][1] == 0) {
+    AF3_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    for (int s = kMaxSplits; s >= 1; --s) {
+      attr[0].val.clusterDim = {(unsigned)s, 1, 1};
+      cfg.gridDim = dim3((unsigned)s, 1024, 1);
+      at_once[dev][s] = clusters_at_once(kern, cfg);
+    }
+  }
+  // The keys are split so that the number of rounds of clusters times the length of one is least:
+  // a CTA takes as long as kFixed keys to begin and to end (5 us against some 150 keys a us), and
+  // half a round is lost at the end when there are several.
+  const int64_t items = (int64_t)a.B * a.hkv;
+  constexpr double kFixed = 768;
+  int splits = 1;
+  double best = 0;
+  for (int s = 1; s <= kMaxSplits; ++s) {
+    const double rounds = (double)items / at_once[dev][s];
+    const double cost = (rounds <= 1 ? 1 : rounds + 0.5) * (kFixed + (double)keys / s);
+    if (s == 1 || cost < best) {
+      best = cost;
+      splits = s;
+    }
+  }
+  cfg.gridDim = dim3((unsigned)splits, (unsigned)a.hkv, (unsigned)a.B);
+  attr[0].val.clusterDim = {(unsigned)splits, 1, 1};
   cfg.numAttrs = splits > 1 ? 1 : 0;
   AF3_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, a, rows_per_tile, splits));
 }
 
 template <bool FP8, bool LONG, bool ONE>
-static void launch_few_t(const Args& a, int max_q, int splits, cudaStream_t stream) {
+static void launch_few_t(const Args& a, int max_q, int64_t keys, cudaStream_t stream) {
   const int want = std::max(std::min(max_q, kFewRows / a.group), 1) * a.group;  // rows of a tile
   if (want <= 8)
-    launch_few_nt<FP8, 1, LONG, ONE>(a, want, splits, stream);
+    launch_few_nt<FP8, 1, LONG, ONE>(a, want, keys, stream);
   else if (want <= 16)
-    launch_few_nt<FP8, 2, LONG, ONE>(a, want, splits, stream);
+    launch_few_nt<FP8, 2, LONG, ONE>(a, want, keys, stream);
   else
-    launch_few_nt<FP8, 4, LONG, ONE>(a, want, splits, stream);
+    launch_few_nt<FP8, 4, LONG, ONE>(a, want, keys, stream);
 }
 
 void launch_few(const Args& a, int64_t max_q, int64_t max_len, cudaStream_t stream) {
   const int64_t keys = a.window > 0 ? std::min<int64_t>(max_len, a.window + max_q) : max_len;
-  const int64_t items = (int64_t)a.B * a.hkv;
-  // The keys are split until there are several CTAs for each SM to even out ragged lengths, as long
-  // as a part has 512 keys (two blocks a warp).  8 CTAs is the largest portable cluster.
-  int splits = 1;
-  const int64_t enough = 4 * (int64_t)num_sms();
-  while (splits < 8 && items * splits < enough && keys >= 512 * splits) splits *= 2;
-  if (getenv("DBG_SPLIT")) splits = atoi(getenv("DBG_SPLIT"));
   const int q = (int)std::min<int64_t>(max_q, kFewRows);
-  const bool is_long = keys > 9 * 32 * splits;  // more than 8 blocks wherever the first one begins
+  // 8 blocks of 32 keys for 4 warps; a part of more in the short shape only runs slower
+  const bool is_long = keys > 256 && (keys > 8 * 256 || (int64_t)a.B * a.hkv * 8 > 3 * (int64_t)num_sms());
   const bool one = (a.p.page_size & 31) == 0;
   auto go = [&](auto fp8, auto lng, auto on) {
-    launch_few_t<decltype(fp8)::value, decltype(lng)::value, decltype(on)::value>(a, q, splits, stream);
+    launch_few_t<decltype(fp8)::value, decltype(lng)::value, decltype(on)::value>(a, q, keys, stream);
   };
   using T = std::true_type;
   using F = std::false_type;
