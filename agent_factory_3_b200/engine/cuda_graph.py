@@ -57,6 +57,7 @@ class _Graph:
         m.ids_t, m.pos_t, m.slots_t = self.ids, self.pos, self.slots
         m.dec_pt, m.dec_lens = self.pt, self.lens
         m.dec_rows = torch.arange(B, device=dev, dtype=torch.long)
+        m.dec_cu = torch.arange(B + 1, device=dev, dtype=torch.int32)
         m.dec_max = chunks * 16 * P
         m.dec_identity = True
         self.m = m

@@ -6,6 +6,9 @@ Pages hold ``page_size`` consecutive tokens of one sequence for every layer (K a
 served from the prefix cache.  Full pages are indexed by a hash chain over their tokens,
 salted with the request's cache key and LoRA adapter; cached pages with no owner are kept in
 LRU order and reclaimed when the free list runs dry.
+
+With ``kv_quant="e4m3"`` the pools hold e4m3 codes and one power-of-two scale byte per token and
+KV head (``ops.paged``): 0.51 of the bf16 bytes, so about twice the tokens per GB.
 """
 from __future__ import annotations
 
@@ -15,6 +18,8 @@ from collections import OrderedDict
 import numpy as np
 import torch
 
+from ..ops import paged
+
 
 class OutOfPages(RuntimeError):
     pass
@@ -23,9 +28,10 @@ class OutOfPages(RuntimeError):
 class PagedKVCache:
     @staticmethod
     def bytes_per_page(num_layers: int, page_size: int, hkv: int, head_dim: int, top_k: int,
-                       elem_bytes: int = 2) -> int:
+                       elem_bytes: int = 2, kv_quant: str | None = None) -> int:
         """Device bytes one page holds: K and V of every layer plus the routed-expert capture."""
-        return num_layers * page_size * (2 * hkv * head_dim * elem_bytes + top_k)
+        row = head_dim + 1 if kv_quant else head_dim * elem_bytes   # codes and a scale byte
+        return num_layers * page_size * (2 * hkv * row + top_k)
 
     @staticmethod
     def pages_for_memory_fraction(fraction: float, total_bytes: int, used_bytes: int,
@@ -42,14 +48,26 @@ class PagedKVCache:
         return pages
 
     def __init__(self, num_layers: int, num_pages: int, page_size: int, hkv: int, head_dim: int,
-                 top_k: int, device, dtype=torch.bfloat16):
+                 top_k: int, device, dtype=torch.bfloat16, kv_quant: str | None = None):
+        if kv_quant not in (None, "e4m3"):
+            raise ValueError(f"kv_quant must be None or 'e4m3', got {kv_quant!r}")
         self.num_layers, self.num_pages, self.page_size = num_layers, num_pages, page_size
         self.hkv, self.head_dim, self.top_k = hkv, head_dim, top_k
         self.device = torch.device(device)
-        self.k = [torch.zeros(num_pages, page_size, hkv, head_dim, device=device, dtype=dtype)
-                  for _ in range(num_layers)]
-        self.v = [torch.zeros(num_pages, page_size, hkv, head_dim, device=device, dtype=dtype)
-                  for _ in range(num_layers)]
+        self.kv_quant = kv_quant
+        self.k_scale: list = [None] * num_layers
+        self.v_scale: list = [None] * num_layers
+        if kv_quant:
+            shape = (num_pages, page_size, hkv, head_dim, device)
+            k = [paged.empty_fp8_pages(*shape) for _ in range(num_layers)]
+            v = [paged.empty_fp8_pages(*shape) for _ in range(num_layers)]
+            self.k, self.k_scale = [c for c, _ in k], [s for _, s in k]
+            self.v, self.v_scale = [c for c, _ in v], [s for _, s in v]
+        else:
+            self.k = [torch.zeros(num_pages, page_size, hkv, head_dim, device=device, dtype=dtype)
+                      for _ in range(num_layers)]
+            self.v = [torch.zeros(num_pages, page_size, hkv, head_dim, device=device, dtype=dtype)
+                      for _ in range(num_layers)]
         self.routing = torch.full((num_pages, page_size, num_layers, top_k), 255, dtype=torch.uint8,
                                   device=device)
         self.refcount = np.zeros(num_pages, dtype=np.int32)
@@ -63,7 +81,8 @@ class PagedKVCache:
     # ------------------------------------------------------------------ accounting
     @property
     def bytes_per_token(self) -> int:
-        return self.num_layers * 2 * self.hkv * self.head_dim * 2
+        return self.num_layers * 2 * self.hkv * (self.head_dim + 1 if self.kv_quant
+                                                 else self.head_dim * 2)
 
     def used_pages(self) -> int:
         return self.num_pages - len(self.free) - len(self.lru)
@@ -73,6 +92,21 @@ class PagedKVCache:
 
     def gb(self) -> float:
         return self.num_pages * self.page_size * self.bytes_per_token / 1e9
+
+    def read(self, layer: int, slots: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        """K and V [n, Hkv, D] of cache slots (page * page_size + offset) of one layer, in bf16
+        (the pool's own type when it is not quantised)."""
+        w = self.hkv * self.head_dim
+        n = slots.numel()
+        if self.kv_quant:
+            rows = torch.zeros(n, 2 * w, device=self.device, dtype=torch.bfloat16)
+            paged.kv_gather_fp8(rows, 0, w, slots.to(self.device), self.k[layer], self.v[layer],
+                                self.k_scale[layer], self.v_scale[layer])
+            k, v = rows[:, :w], rows[:, w:]
+        else:
+            at = slots.to(self.device).long()
+            k, v = (p.view(-1, w).index_select(0, at) for p in (self.k[layer], self.v[layer]))
+        return k.reshape(n, self.hkv, self.head_dim), v.reshape(n, self.hkv, self.head_dim)
 
     # ------------------------------------------------------------------ hashing
     @staticmethod

@@ -6,6 +6,9 @@ once per layer for the whole batch.  Attention splits by kind:
   * prefill chunks -> the packed flash-attention kernel on a buffer holding each sequence's
     full context (cached K/V gathered from pages, queries only for the new rows; the tile list
     covers just the new rows).
+With ``paged`` (always so for a quantised cache) both kinds, and speculative verify blocks, attend
+to the pages in place instead (``ops.paged.paged_attention``): no context is gathered, and a verify
+block reads its context once rather than once per draft token.
 New K/V go straight into their page slots; the MoE expert ids chosen for every new token are
 written next to them so routed experts can be returned for prefix-cache hits later.
 """
@@ -18,6 +21,7 @@ import torch
 
 from ..models.gpt_oss.model import GptOssForCausalLM
 from ..ops import decode as D
+from ..ops import paged as P8
 from ..ops._ext import ext, use_cuda_kernels
 from ..ops.attention import attention_reference
 from ..ops.gemm import matmul
@@ -47,15 +51,22 @@ class StepOutput:
 
 
 class ModelRunner:
-    def __init__(self, model: GptOssForCausalLM, kv: PagedKVCache, lora_active: bool = True):
+    def __init__(self, model: GptOssForCausalLM, kv: PagedKVCache, lora_active: bool = True,
+                 paged: bool = False):
         self.model = model
         self.kv = kv
+        self.paged = paged or kv.kv_quant is not None
         self.cfg = model.cfg
         self.lora_active = lora_active
         self.device = model.embed_tokens.device
         self._bd_cache: dict = {}
         self._multi_cache: dict = {}
         self.graphs = None      # engine.cuda_graph.DecodeGraphs when decode steps are captured
+
+    def _pages_in_place(self) -> bool:
+        """Whether prefill chunks attend to the pages themselves: with ``paged``, where the head
+        dimension is the kernel's."""
+        return self.paged and (self.cfg.head_dim == 64 or self.device.type != "cuda")
 
     def _qkv_lora(self, attn):
         if not self.lora_active:
@@ -81,7 +92,7 @@ class ModelRunner:
             rows.append((r0, r0 + n))
             # a speculative verify block on top of cached pages is decoded row by row: its K/V
             # are stored first, so token j attends to start + j + 1 cached positions
-            decode = it.start > 0 and (n == 1 or it.all_logits)
+            decode = it.start > 0 and (n == 1 or (it.all_logits and not self.paged))
             (dec_idx if decode else pre_idx).append(i)
         m.N, m.rows, m.dec_idx, m.pre_idx = len(ids), rows, dec_idx, pre_idx
         m.ids_t = torch.tensor(ids, device=dev, dtype=torch.long)
@@ -103,9 +114,27 @@ class ModelRunner:
             m.dec_pt = pt.to(dev)
             m.dec_lens = torch.tensor(lens, device=dev, dtype=torch.int32)
             m.dec_rows = torch.tensor(drows, device=dev, dtype=torch.long)
+            m.dec_cu = torch.arange(n_dec + 1, device=dev, dtype=torch.int32)
             m.dec_max = int(max(lens))
             m.dec_identity = (not pre_idx) and drows == list(range(len(ids)))
-        if pre_idx:   # packed full contexts of the prefill chunks
+        m.pre_paged = bool(pre_idx) and self._pages_in_place()
+        if m.pre_paged:   # chunks read the pages: tables, lengths and row ranges
+            its = [items[i] for i in pre_idx]
+            pt = torch.zeros(len(its), max(len(it.pages) for it in its), dtype=torch.int32)
+            for r, it in enumerate(its):
+                pt[r, :len(it.pages)] = torch.tensor(it.pages, dtype=torch.int32)
+            cu = [0]
+            for it in its:
+                cu.append(cu[-1] + len(it.ids))
+            m.pre_pt = pt.to(dev)
+            m.pre_lens = torch.tensor([it.start + len(it.ids) for it in its], dtype=torch.int32).to(dev)
+            m.pre_cu = torch.tensor(cu, dtype=torch.int32).to(dev)
+            m.pre_max_q = max(len(it.ids) for it in its)
+            m.pre_max = max(it.start + len(it.ids) for it in its)
+            if dec_idx:
+                m.new_rows_t = torch.tensor([r for i in pre_idx for r in range(*rows[i])],
+                                            device=dev, dtype=torch.long)
+        elif pre_idx:   # packed full contexts of the prefill chunks
             ctx_slots, new_in_ctx, new_rows, tiles, cu = [], [], [], [], [0]
             for i in pre_idx:
                 it = items[i]
@@ -141,21 +170,40 @@ class ModelRunner:
         else:
             qkv = lora_linear(xn, qkv_w, qkv_b, A, B, None, lora_s)
         apply_rope_(qkv, hq + hkv, d, m.pos_t, cos, sin)
-        kp, vp = self.kv.k[li], self.kv.v[li]
-        D.kv_store(qkv, qs, qs + kvs, m.slots_t, kp, vp)
+        kp, vp, ksc, vsc = self.kv.k[li], self.kv.v[li], self.kv.k_scale[li], self.kv.v_scale[li]
+        if ksc is not None:
+            P8.kv_store_fp8(qkv, qs, qs + kvs, m.slots_t, kp, vp, ksc, vsc)
+        else:
+            D.kv_store(qkv, qs, qs + kvs, m.slots_t, kp, vp)
+
+        def decode(q):
+            if self.paged:
+                return P8.paged_attention(q, kp, vp, m.dec_pt, m.dec_lens, m.dec_cu, sinks, hq, hkv,
+                                          window, scale, ksc, vsc, 1, m.dec_max)
+            return D.decode_attention(q, kp, vp, m.dec_pt, m.dec_lens, sinks, hq, hkv, window, scale,
+                                      m.dec_max)
+
+        def chunks(q):
+            return P8.paged_attention(q, kp, vp, m.pre_pt, m.pre_lens, m.pre_cu, sinks, hq, hkv,
+                                      window, scale, ksc, vsc, m.pre_max_q, m.pre_max)
+
         if m.dec_idx and not m.pre_idx and getattr(m, "dec_identity", False):
             # every row is a decode row, in order: no gather / scatter around the kernel
-            return D.decode_attention(qkv[:, :qs], kp, vp, m.dec_pt, m.dec_lens, sinks, hq, hkv,
-                                      window, scale, m.dec_max)
+            return decode(qkv[:, :qs])
+        if m.pre_idx and not m.dec_idx and m.pre_paged:
+            return chunks(qkv[:, :qs])
         o = torch.empty(m.N, qs, device=dev, dtype=qkv.dtype)
         if m.dec_idx:
             q = qkv.index_select(0, m.dec_rows)
-            od = D.decode_attention(q[:, :qs], kp, vp, m.dec_pt, m.dec_lens, sinks, hq, hkv,
-                                    window, scale, m.dec_max)
-            o.index_copy_(0, m.dec_rows, od)
-        if m.pre_idx:
+            o.index_copy_(0, m.dec_rows, decode(q[:, :qs]))
+        if m.pre_idx and m.pre_paged:
+            o.index_copy_(0, m.new_rows_t, chunks(qkv.index_select(0, m.new_rows_t)[:, :qs]))
+        elif m.pre_idx:
             ctx = torch.zeros(m.n_ctx, qkv.shape[1], device=dev, dtype=qkv.dtype)
-            D.kv_gather(ctx, qs, qs + kvs, m.ctx_slots_t, kp, vp)
+            if ksc is not None:
+                P8.kv_gather_fp8(ctx, qs, qs + kvs, m.ctx_slots_t, kp, vp, ksc, vsc)
+            else:
+                D.kv_gather(ctx, qs, qs + kvs, m.ctx_slots_t, kp, vp)
             ctx.index_copy_(0, m.new_in_ctx_t, qkv.index_select(0, m.new_rows_t))
             if use_cuda_kernels(ctx) and d == 64:
                 oc = torch.empty(m.n_ctx, qs, device=dev, dtype=qkv.dtype)

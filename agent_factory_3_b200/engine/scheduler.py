@@ -80,21 +80,25 @@ class Engine:
     def __init__(self, model, *, num_pages: int = 4096, page_size: int = 64,
                  max_running: int = 128, max_prefill_tokens: int = 16384,
                  max_context_tokens: Optional[int] = None, weight_version: str = "0",
-                 tp=None, tp_shards=None, drafter=None, cuda_graphs: Optional[bool] = None):
+                 tp=None, tp_shards=None, drafter=None, cuda_graphs: Optional[bool] = None,
+                 kv_quant: Optional[str] = None, paged_attention: bool = False):
         """``tp``: an ``engine.tp.TPContext`` to run tensor-parallel (this process is one rank;
-        rank 0 runs the scheduler, the others call ``self.runner.follow()``)."""
+        rank 0 runs the scheduler, the others call ``self.runner.follow()``).  ``kv_quant``:
+        "e4m3" keeps the KV cache in 8 bits.  ``paged_attention``: prefill chunks, verify blocks
+        and decode rows attend to the cache pages in place (implied by ``kv_quant``)."""
         self.model = model
         cfg = model.cfg
         dev = model.embed_tokens.device
         world = tp.world if tp is not None else 1
         self.kv = PagedKVCache(cfg.num_hidden_layers, num_pages, page_size,
                                cfg.num_key_value_heads // world, cfg.head_dim,
-                               cfg.num_experts_per_tok, dev, dtype=model.embed_tokens.dtype)
+                               cfg.num_experts_per_tok, dev, dtype=model.embed_tokens.dtype,
+                               kv_quant=kv_quant)
         if tp is not None:
             from .tp import TPModelRunner
-            self.runner = TPModelRunner(model, self.kv, tp, tp_shards)
+            self.runner = TPModelRunner(model, self.kv, tp, tp_shards, paged=paged_attention)
         else:
-            self.runner = ModelRunner(model, self.kv, lora_active=False)
+            self.runner = ModelRunner(model, self.kv, lora_active=False, paged=paged_attention)
             if cuda_graphs is None:
                 cuda_graphs = os.environ.get("AF3_CUDA_GRAPHS") == "1"
             if cuda_graphs and dev.type == "cuda":

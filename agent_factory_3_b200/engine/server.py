@@ -246,7 +246,13 @@ def build_arg_parser() -> argparse.ArgumentParser:
     ap.add_argument("--dtype", default="bfloat16", choices=["auto", "bfloat16", "bf16"])
     ap.add_argument("--kv-cache-dtype", default="auto",
                     choices=["auto", "bfloat16", "bf16", "fp8_e4m3", "fp8_e5m2"],
-                    help="the KV cache is bf16; fp8 requests are accepted and noted")
+                    help="bf16; fp8 requests are accepted and noted (see --kv-quant)")
+    ap.add_argument("--kv-quant", default="none", choices=["none", "e4m3"],
+                    help="e4m3: KV cache in 8 bits, one power-of-two scale per token and KV head "
+                         "(half the memory per cached token)")
+    ap.add_argument("--paged-attention", action="store_true",
+                    help="attend to the cache pages in place in prefill, verify and decode "
+                         "(implied by --kv-quant)")
     ap.add_argument("--speculative-algorithm", type=str.lower, default="none",
                     choices=["none", "block", "ngram", "dflash"],
                     help="block (alias dflash): one-forward block draft model sharing the "
@@ -275,8 +281,9 @@ def resolve_args(a: argparse.Namespace, world: int) -> list[str]:
     if a.speculative_algorithm == "dflash":
         a.speculative_algorithm = "block"
         notes.append(f"DFLASH -> block draft of {a.speculative_num_draft_tokens} tokens")
-    if a.kv_cache_dtype.startswith("fp8"):
-        notes.append(f"--kv-cache-dtype {a.kv_cache_dtype}: the KV cache stays bf16")
+    if a.kv_cache_dtype.startswith("fp8") and a.kv_quant == "none":
+        notes.append(f"--kv-cache-dtype {a.kv_cache_dtype}: the KV cache stays bf16 "
+                     "(--kv-quant e4m3 keeps it in 8 bits)")
     if a.speculative_draft_model_path:
         notes.append("--speculative-draft-model-path: the block draft is built from the target")
     if a.num_pages is not None and a.mem_fraction_static is not None:
@@ -340,7 +347,8 @@ def main():
         free, total = torch.cuda.mem_get_info(dev)
         page_bytes = PagedKVCache.bytes_per_page(cfg.num_hidden_layers, a.page_size,
                                                  cfg.num_key_value_heads // world, cfg.head_dim,
-                                                 cfg.num_experts_per_tok)
+                                                 cfg.num_experts_per_tok,
+                                                 kv_quant=None if a.kv_quant == "none" else a.kv_quant)
         num_pages = PagedKVCache.pages_for_memory_fraction(a.mem_fraction_static, total,
                                                            total - free, page_bytes)
         if rank == 0:
@@ -349,7 +357,9 @@ def main():
     eng = Engine(model, num_pages=num_pages, page_size=a.page_size,
                  max_running=a.max_running_requests, max_prefill_tokens=a.max_prefill_tokens,
                  tp=tp, tp_shards=shards, drafter=drafter,
-                 cuda_graphs=a.cuda_graphs and world == 1)
+                 cuda_graphs=a.cuda_graphs and world == 1,
+                 kv_quant=None if a.kv_quant == "none" else a.kv_quant,
+                 paged_attention=a.paged_attention)
     if rank != 0:
         eng.runner.follow()
         tp.shutdown()

@@ -315,8 +315,9 @@ class TPModelRunner(ModelRunner):
     factors are broadcast over the device group into every rank's model and each rank keeps its
     slices (``shard_lora``).  Every step message carries whether the adapter is active."""
 
-    def __init__(self, model, kv, ctx: TPContext, shards: list[LayerShard] | None = None):
-        super().__init__(model, kv, lora_active=False)
+    def __init__(self, model, kv, ctx: TPContext, shards: list[LayerShard] | None = None,
+                 paged: bool = False):
+        super().__init__(model, kv, lora_active=False, paged=paged)
         self.ctx = ctx
         self.shards = shards if shards is not None else shard_model(model, ctx.rank, ctx.world)
         self.lora_shards: list[LoraShard] | None = None
