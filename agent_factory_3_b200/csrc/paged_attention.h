@@ -11,6 +11,8 @@ constexpr int kFewRows = 32;  // query rows a KV head that launch_few takes in o
 // powers of two, f16 no longer holds all of them well enough once a row does not see the largest;
 // such a tile's rows are taken key by key.  Tokens of one sequence differ by far less.
 constexpr int kWideRange = 14;
+// bf16 V scaled to f16 keeps 2^-25 of 2^8; judged by 8 values at a time.
+constexpr int kWideRangeBf16 = 18;
 
 // At most kFewRows query rows a KV head and sequence: memory-bound, split over the keys.
 void launch_few(const Args& a, int64_t max_q, int64_t max_len, cudaStream_t stream);

@@ -28,93 +28,113 @@ struct RowArgs {
   uint32_t n_slots;
 };
 
-// One warp per (row of qkv, K or V); the warp's lanes walk the row's Hkv * D / 8 pieces.
+// One warp per row of qkv; its lanes walk the row's Hkv * D / 8 pieces of K and of V, 32 at a time.
+// The loads of both go out before anything waits, for the slot too.
 __global__ void __launch_bounds__(kCacheThreads) kv_store_fp8_kernel(const RowArgs a, const Pool p) {
-  const int task = (blockIdx.x * kCacheThreads + threadIdx.x) >> 5, lane = threadIdx.x & 31;
-  const int row = task >> 1;
-  const bool is_v = task & 1;
+  const int row = (blockIdx.x * kCacheThreads + threadIdx.x) >> 5, lane = threadIdx.x & 31;
   if (row >= a.n) return;
   const uint32_t slot = (uint32_t)a.slots[row];
-  if (slot >= a.n_slots) return;  // negative or past the pool
-  uint32_t page, off;
-  split_slot(p, slot, page, off);
-  const uint4* src = reinterpret_cast<const uint4*>(a.qkv + (int64_t)row * a.ld + (is_v ? a.v_off : a.k_off));
-  uint8_t* dst = (is_v ? p.v : p.k) + (int64_t)page * p.page + (int64_t)off * p.token;
-  uint8_t* sdst = (is_v ? p.vs : p.ks) + (int64_t)page * p.s_page + (int64_t)off * p.s_token;
+  const __nv_bfloat16* src = a.qkv + (int64_t)row * a.ld;
+  const uint4* from[2] = {reinterpret_cast<const uint4*>(src + a.k_off), reinterpret_cast<const uint4*>(src + a.v_off)};
   const int pieces = a.hkv << a.lanes_log2, per_row = 1 << a.lanes_log2;
-  for (int base = 0; base < pieces; base += 32) {
-    const int i = base + lane;
-    const bool on = i < pieces;  // a row's lanes are all on or all off: per_row divides 32
-    const uint4 w = on ? src[i] : make_uint4(0u, 0u, 0u, 0u);
-    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&w);
-    float x[8];
-    float amax = 0.f;
+  for (int base = 0; base < pieces; base += 64) {
+    uint4 w[4];  // K, V of piece base + lane, then of base + 32 + lane
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 f = __bfloat1622float2(h[j]);
-      x[2 * j] = f.x;
-      x[2 * j + 1] = f.y;
+    for (int u = 0; u < 4; ++u) {
+      const int i = base + 32 * (u >> 1) + lane;
+      w[u] = i < pieces ? __ldcs(from[u & 1] + i) : make_uint4(0u, 0u, 0u, 0u);
     }
+    if (slot >= a.n_slots) return;  // negative or past the pool
+    uint32_t page, off;
+    split_slot(p, slot, page, off);
+    const int64_t at = (int64_t)page * p.page + (int64_t)off * p.token;
+    const int64_t sat = (int64_t)page * p.s_page + (int64_t)off * p.s_token;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float m = fabsf(x[j]);
-      if (m < INFINITY) amax = fmaxf(amax, m);  // false for NaN
-    }
-    for (int o = per_row >> 1; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    const uint32_t bits = __float_as_uint(amax);
-    // a = 1.m * 2^E <= 448 * 2^e = 1.75 * 2^(e + 8)
-    int e = (int)(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
-    e = min(max(e, -127), 120);
-    const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
-    const float lim = e == 120 ? 240.f : 448.f;
-    uint32_t out[2];
+    for (int u = 0; u < 4; ++u) {
+      const int i = base + 32 * (u >> 1) + lane;
+      const bool on = i < pieces;  // a row's lanes are all on or all off: per_row divides 32
+      const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&w[u]);
+      float x[8];
+      float amax = 0.f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const bool fin = fabsf(x[j]) < INFINITY;
-      x[j] = fin ? fminf(fmaxf(x[j] * inv, -lim), lim) : __uint_as_float(0x7fc00000u);
-    }
+      for (int j = 0; j < 4; ++j) {
+        const float2 f = __bfloat1622float2(h[j]);
+        x[2 * j] = f.x;
+        x[2 * j + 1] = f.y;
+      }
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      uint16_t lo, hi;
-      asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(x[4 * j + 1]), "f"(x[4 * j]));
-      asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(x[4 * j + 3]), "f"(x[4 * j + 2]));
-      out[j] = (uint32_t)lo | ((uint32_t)hi << 16);
-    }
-    if (on) {
-      const int head = i >> a.lanes_log2, piece = i & (per_row - 1);
-      *reinterpret_cast<uint2*>(dst + head * p.head + piece * 8) = make_uint2(out[0], out[1]);
-      if (piece == 0) sdst[head * p.s_head] = (uint8_t)(e + 127);
+      for (int j = 0; j < 8; ++j) {
+        const float m = fabsf(x[j]);
+        if (m < INFINITY) amax = fmaxf(amax, m);  // false for NaN
+      }
+      for (int o = per_row >> 1; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+      const uint32_t bits = __float_as_uint(amax);
+      // a = 1.m * 2^E <= 448 * 2^e = 1.75 * 2^(e + 8)
+      int e = (int)(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+      e = min(max(e, -127), 120);
+      const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
+      const float lim = e == 120 ? 240.f : 448.f;
+      uint32_t out[2];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const bool fin = fabsf(x[j]) < INFINITY;
+        x[j] = fin ? fminf(fmaxf(x[j] * inv, -lim), lim) : __uint_as_float(0x7fc00000u);
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        uint16_t lo, hi;
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(x[4 * j + 1]), "f"(x[4 * j]));
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(x[4 * j + 3]), "f"(x[4 * j + 2]));
+        out[j] = (uint32_t)lo | ((uint32_t)hi << 16);
+      }
+      if (on) {
+        const int head = i >> a.lanes_log2, piece = i & (per_row - 1);
+        *reinterpret_cast<uint2*>(((u & 1) ? p.v : p.k) + at + head * p.head + piece * 8) = make_uint2(out[0], out[1]);
+        if (piece == 0) ((u & 1) ? p.vs : p.ks)[sat + head * p.s_head] = (uint8_t)(e + 127);
+      }
     }
   }
 }
 
+// One warp per row of qkv, 64 pieces of K and of V at a time, every load before the first store.
 __global__ void __launch_bounds__(kCacheThreads) kv_gather_fp8_kernel(const RowArgs a, const Pool p) {
-  const int task = (blockIdx.x * kCacheThreads + threadIdx.x) >> 5, lane = threadIdx.x & 31;
-  const int row = task >> 1;
-  const bool is_v = task & 1;
+  const int row = (blockIdx.x * kCacheThreads + threadIdx.x) >> 5, lane = threadIdx.x & 31;
   if (row >= a.n) return;
   const uint32_t slot = (uint32_t)a.slots[row];
   if (slot >= a.n_slots) return;
   uint32_t page, off;
   split_slot(p, slot, page, off);
-  uint4* dst = reinterpret_cast<uint4*>(a.qkv + (int64_t)row * a.ld + (is_v ? a.v_off : a.k_off));
-  const uint8_t* src = (is_v ? p.v : p.k) + (int64_t)page * p.page + (int64_t)off * p.token;
-  const uint8_t* ssrc = (is_v ? p.vs : p.ks) + (int64_t)page * p.s_page + (int64_t)off * p.s_token;
+  __nv_bfloat16* dst = a.qkv + (int64_t)row * a.ld;
+  uint4* to[2] = {reinterpret_cast<uint4*>(dst + a.k_off), reinterpret_cast<uint4*>(dst + a.v_off)};
+  const int64_t at = (int64_t)page * p.page + (int64_t)off * p.token;
+  const int64_t sat = (int64_t)page * p.s_page + (int64_t)off * p.s_token;
   const int pieces = a.hkv << a.lanes_log2, per_row = 1 << a.lanes_log2;
-  for (int i = lane; i < pieces; i += 32) {
-    const int head = i >> a.lanes_log2, piece = i & (per_row - 1);
-    const uint2 c = *reinterpret_cast<const uint2*>(src + head * p.head + piece * 8);
-    const float s = pow2i((int)ssrc[head * p.s_head] - 127);
-    uint4 w;
-    uint32_t* o = reinterpret_cast<uint32_t*>(&w);
+  for (int base = 0; base < pieces; base += 64) {
+    uint2 c[4];
+    uint32_t byte[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t word = j < 2 ? c.x : c.y;
-      const float2 f = f16x2_to_float2(e4m3x2_to_f16x2((uint16_t)(word >> (16 * (j & 1)))));
-      const __nv_bfloat162 r = __floats2bfloat162_rn(f.x * s, f.y * s);
-      o[j] = *reinterpret_cast<const uint32_t*>(&r);
+    for (int u = 0; u < 4; ++u) {
+      const int i = base + 32 * (u >> 1) + lane;
+      const bool on = i < pieces;
+      const int head = i >> a.lanes_log2, piece = i & (per_row - 1);
+      c[u] = make_uint2(0u, 0u);
+      if (on) c[u] = __ldg(reinterpret_cast<const uint2*>(((u & 1) ? p.v : p.k) + at + head * p.head + piece * 8));
+      byte[u] = load_byte(((u & 1) ? p.vs : p.ks) + sat + head * p.s_head, on);
     }
-    dst[i] = w;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int i = base + 32 * (u >> 1) + lane;
+      const float s = pow2i((int)byte[u] - 127);
+      uint32_t o[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t word = j < 2 ? c[u].x : c[u].y;
+        const float2 f = f16x2_to_float2(e4m3x2_to_f16x2((uint16_t)(word >> (16 * (j & 1)))));
+        const __nv_bfloat162 r = __floats2bfloat162_rn(f.x * s, f.y * s);
+        o[j] = *reinterpret_cast<const uint32_t*>(&r);
+      }
+      if (i < pieces) __stcs(to[u & 1] + i, make_uint4(o[0], o[1], o[2], o[3]));
+    }
   }
 }
 
@@ -160,7 +180,7 @@ void kv_store_fp8(torch::Tensor qkv, int64_t k_off, int64_t v_off, torch::Tensor
   const RowArgs a = row_args(qkv, k_off, v_off, slots, k_pages);
   if (a.n == 0) return;
   const c10::cuda::CUDAGuard guard(qkv.device());
-  const unsigned blocks = (unsigned)((2 * (int64_t)a.n * 32 + kCacheThreads - 1) / kCacheThreads);
+  const unsigned blocks = (unsigned)(((int64_t)a.n * 32 + kCacheThreads - 1) / kCacheThreads);
   kv_store_fp8_kernel<<<blocks, kCacheThreads, 0, at::cuda::getCurrentCUDAStream()>>>(a, p);
   AF3_CUDA_CHECK(cudaGetLastError());
 }
@@ -174,7 +194,7 @@ void kv_gather_fp8(torch::Tensor qkv, int64_t k_off, int64_t v_off, torch::Tenso
   const RowArgs a = row_args(qkv, k_off, v_off, slots, k_pages);
   if (a.n == 0) return;
   const c10::cuda::CUDAGuard guard(qkv.device());
-  const unsigned blocks = (unsigned)((2 * (int64_t)a.n * 32 + kCacheThreads - 1) / kCacheThreads);
+  const unsigned blocks = (unsigned)(((int64_t)a.n * 32 + kCacheThreads - 1) / kCacheThreads);
   kv_gather_fp8_kernel<<<blocks, kCacheThreads, 0, at::cuda::getCurrentCUDAStream()>>>(a, p);
   AF3_CUDA_CHECK(cudaGetLastError());
 }

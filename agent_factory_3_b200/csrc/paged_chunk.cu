@@ -10,6 +10,7 @@
 //   warps 4-11   softmax, one warpgroup per 128-row tile: thread t owns query row t
 //   warp 12      tcgen05 issuer: S = Q K^T (M 128, N 128, K 64) of the next block is issued before
 //                O += P V (M 128, N 64, K 128, P from TMEM) of this one
+//   warps 14-15  bf16 pages: loaders of K, whose rows go straight into their tile
 // TMEM columns: S[A] 0, S[B] 128, P[A] 256, P[B] 320 (f16 pairs), O[A] 384, O[B] 448.
 //
 // P and V enter the second product as f16: bf16's 8 bits for P would cost as much precision as the
@@ -18,8 +19,8 @@
 //   e4m3 pages: V' = code * 2^(e - u), K' = code * 2^(e - ek) with ek the block's largest exponent;
 //               both exact while a key's exponent is within kWideRange of the largest
 //   bf16 pages: V' = v * 2^-u with the largest |V'| in [2^8, 2^9); K and Q stay bf16
-// The softmax reference moves only when a score passes it by 2^8; P is in (0, 2^14].  The row sum
-// adds the rounded P, so that a row that one key dominates comes out as that key's value.
+// The softmax reference is the running maximum itself: the largest p is 2^10 exactly, so that a row
+// that one key dominates comes out as that key's value, and f16 keeps 11 bits down to 2^-24 of it.
 //
 // Rows that do not see a value must not meet it as 0 * inf: blocks that are not fully visible to
 // the whole span have such values cleared by the loaders and their keys reported; rows that do see
@@ -42,7 +43,7 @@ constexpr int kST = 4;           // f16 K/V stages
 constexpr int kRaw = 3;          // raw blocks in flight
 constexpr int kTile = kBK * kD * 2;  // 16 KB: a 16-bit K, V or Q tile; also a raw block
 constexpr uint32_t kColS = 0, kColP = 256, kColO = 384;
-constexpr float kTopLog2 = 10.f, kGrowLog2 = 0.f;
+constexpr float kTopLog2 = 10.f;  // the largest p of a row is 2^10
 
 struct ChunkSmem {
   static constexpr int Q = 0;                    // 2 tiles
@@ -56,7 +57,7 @@ struct ChunkSmem {
 struct StageInfo {
   uint32_t there[4];   // keys that exist and lie in the span's range
   uint32_t broken[4];  // keys whose V is not finite (cleared), in blocks not seen by every row
-  float kmul;          // 2^ek
+  float kmul;          // 2^ek (e4m3)
   int unit;            // V' is in units of 2^unit
 };
 
@@ -65,7 +66,7 @@ struct ChunkBars {
   uint32_t tmem;
   int abort_flag;
   int wide;
-  uint32_t red[2][4][2];
+  uint32_t red[2][4];
   StageInfo info[kST];
   float row_m[256], row_l[256];
 };
@@ -105,12 +106,6 @@ __device__ __forceinline__ uint32_t h2_of(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
-}
-// s0 += low half of w, s1 += high half
-__device__ __forceinline__ void add_h2(float& s0, float& s1, uint32_t w) {
-  asm("{\n.reg .f16 l, h;\nmov.b32 {l, h}, %2;\nadd.rn.f32.f16 %0, l, %0;\nadd.rn.f32.f16 %1, h, %1;\n}"
-      : "+f"(s0), "+f"(s1)
-      : "r"(w));
 }
 __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
   uint32_t r;
@@ -199,9 +194,9 @@ __device__ __forceinline__ bool issue_pv(Issue& t, int j, int st, uint32_t tmem,
   return true;
 }
 
-// ------------------------------------------------------------------------------- loader
-// Rows of a block: warp w has keys [32 w, 32 w + 32); lane l looks up key 32 w + l.
-struct Ahead {
+// ------------------------------------------------------------------------------- loaders
+// A warp loads rows in groups of 32 keys; lane l looks up the group's key l.
+struct Rows {
   uint32_t there;
   int64_t scale;  // offset of the lane's scale bytes
 };
@@ -214,47 +209,49 @@ __device__ __forceinline__ int page_of(const Args& a, const int* table, int j, i
   return page;
 }
 
-template <bool FP8>
-__device__ __forceinline__ Ahead load_block(const Args& a, int page, int g, int k0, int w, int lane, uint32_t raw,
-                                            uint32_t kdst) {
+// Starts the copies of keys key0 .. key0 + 31 of `pool`: piece i of lane l, rows 8 i + l / 4 (e4m3,
+// 16 codes each) or 4 i + l / 8 (bf16, 8 values), goes to own + i * pitch (and `pool2`'s pieces after
+// `pool`'s, e4m3), or with TILE into rows r0 .. r0 + 31 of a swizzled tile.
+template <bool FP8, bool TILE>
+__device__ __forceinline__ Rows load_rows(const Args& a, const uint8_t* pool, const uint8_t* pool2, int page, int g, int key0,
+                                          uint32_t dst, int pitch_or_r0) {
+  const int lane = threadIdx.x & 31;
   const bool on = (uint32_t)page < (uint32_t)a.p.num_pages;
   int64_t row = 0, sc = 0;
   if (on) {
     uint32_t pi, off;
-    split_slot(a.p, (uint32_t)(k0 + 32 * w + lane), pi, off);
+    split_slot(a.p, (uint32_t)(key0 + lane), pi, off);
     row = (int64_t)page * a.p.page + (int64_t)off * a.p.token + (int64_t)g * a.p.head;
     sc = (int64_t)page * a.p.s_page + (int64_t)off * a.p.s_token + (int64_t)g * a.p.s_head;
   }
-  Ahead h;
+  Rows h;
   h.there = __ballot_sync(0xffffffffu, on);
   h.scale = sc;
-  const uint32_t own = raw + (32 * w + lane) * 16;
-  if constexpr (FP8) {  // K pieces 0-3, V pieces 4-7, 16 codes each
-    const int c = lane & 3;
+  constexpr int kPer = FP8 ? 4 : 8;  // pieces of a row = rows a piece index steps over, inverted
+  const int c = lane % kPer;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = 8 * i + (lane >> 2);
-      const int64_t off = __shfl_sync(0xffffffffu, row, r) + c * 16;
-      const bool there = (h.there >> r) & 1u;
-      cp16(own + i * 2048, a.p.k + off, there);
-      cp16(own + (4 + i) * 2048, a.p.v + off, there);
-    }
-  } else {  // K straight into its tile, V pieces 0-7
-    const int c = lane & 7;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int r = 4 * i + (lane >> 3);
-      const int64_t off = __shfl_sync(0xffffffffu, row, r) + c * 16;
-      const bool there = (h.there >> r) & 1u;
-      cp16(kdst + sw128(32 * w + r, c), a.p.k + off, there);
-      cp16(own + i * 2048, a.p.v + off, there);
+  for (int i = 0; i < kPer; ++i) {
+    const int r = (32 / kPer) * i + lane / kPer;
+    const int64_t off = __shfl_sync(0xffffffffu, row, r) + c * 16;
+    const bool there = (h.there >> r) & 1u;
+    if constexpr (TILE) {
+      cp16(dst + sw128(pitch_or_r0 + r, c), pool + off, there);
+    } else {
+      cp16(dst + i * pitch_or_r0, pool + off, there);
+      if constexpr (FP8) cp16(dst + (4 + i) * pitch_or_r0, pool2 + off, there);
     }
   }
   return h;
 }
 
+// Bits at 0, n, 2 n, ... of x: whether any of the n lanes from there on has its bit set.
+__device__ __forceinline__ uint32_t any_of_groups(uint32_t x, int n) {
+  for (int s = 1; s < n; s *= 2) x |= x >> s;
+  return x & (n == 4 ? 0x11111111u : 0x01010101u);
+}
+
 __device__ __forceinline__ void st4(uint32_t addr, uint32_t x, uint32_t y, uint32_t z, uint32_t u) {
-  st_shared_v4(addr, x, y, z, u);
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(u));
 }
 
 // 16 e4m3 codes -> 16 f16 scaled by mul, into chunks 2c and 2c + 1 of row r.
@@ -305,7 +302,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
   if (warp == 0 && lane == 0) {
     mbar_init(&b->q_full, 8);
     for (int s = 0; s < kST; ++s) {
-      mbar_init(&b->kv_full[s], 4);
+      mbar_init(&b->kv_full[s], FP8 ? 4 : 6);
       mbar_init(&b->kv_empty[s], 1);
     }
     for (int x = 0; x < 2; ++x) {
@@ -328,93 +325,93 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
   const uint32_t tmem = b->tmem;
   const uint32_t sbase = smem_u32(smem);
 
-  // registers (launch: 512 x 128): loaders 88, softmax 2 x 192, issuer 40: 512 x 128 in all
+  // a block is seen in full by every row of the span when it lies in [full_lo, full_hi)
+  const int full_lo = a.window > 0 ? pos0 + ntok - a.window : 0, full_hi = min(pos0 + 1, sq.key_end);
+
+  // registers (launch: 512 x 128): loaders 72, softmax 2 x 184, issuer and K loaders 72
   if (warp < 4) {
-    setmaxnreg_dec<88>();
+    setmaxnreg_dec<72>();
     const int w = warp;
-    // a block is seen in full by every row of the span when it lies in [full_lo, full_hi)
-    const int full_lo = a.window > 0 ? pos0 + ntok - a.window : 0, full_hi = min(pos0 + 1, sq.key_end);
-    uint32_t top = 0;  // V: largest e8m0 byte (e4m3) or biased exponent (bf16) so far
+    constexpr int kPieces = FP8 ? 4 : 8;
+    uint32_t top = 0;  // largest e8m0 byte (e4m3) or biased exponent (bf16) so far
     bool dead = false;
-    Ahead ah[kRaw];
-    // scale bytes of the next block to expand, as loaded: combining them here would wait for them
-    uint32_t next_k = 0, next_v = 0;
-    auto fetch_scales = [&](const Ahead& h) {
-      if constexpr (FP8) {
-        next_k = load_byte(a.p.ks + h.scale, (h.there >> lane) & 1u);
-        next_v = load_byte(a.p.vs + h.scale, (h.there >> lane) & 1u);
-      }
+    Rows ah[kRaw];
+    // scale bytes of the next two blocks, loaded two blocks before they are used
+    uint32_t byte0 = 0, byte1 = 0, kbyte0 = 0, kbyte1 = 0;
+    auto fetch_scale = [&](const uint8_t* from, const Rows& h) -> uint32_t {
+      return FP8 ? load_byte(from + h.scale, (h.there >> lane) & 1u) : 0u;
     };
-    const int lane_key = lo + 32 * w + lane;
-    int first_pages[kRaw];
+    const int key0 = lo + 32 * w;
+    int pages[kRaw];
 #pragma unroll
-    for (int i = 0; i < kRaw; ++i) first_pages[i] = b0 + i < b1 ? page_of(a, table, lane_key + (b0 + i) * kBK, hi) : -1;
-    int next_page = b0 + kRaw < b1 ? page_of(a, table, lane_key + (b0 + kRaw) * kBK, hi) : -1;
+    for (int i = 0; i < kRaw; ++i) pages[i] = b0 + i < b1 ? page_of(a, table, key0 + lane + (b0 + i) * kBK, hi) : -1;
+    int next_page = b0 + kRaw < b1 ? page_of(a, table, key0 + lane + (b0 + kRaw) * kBK, hi) : -1;
+    const uint32_t own0 = sbase + ChunkSmem::RAW + (32 * w + lane) * 16;
 #pragma unroll
     for (int i = 0; i < kRaw; ++i) {
-      ah[i].there = 0;
-      ah[i].scale = 0;
-      if (b0 + i < b1)
-        ah[i] = load_block<FP8>(a, first_pages[i], g, lo + (b0 + i) * kBK, w, lane, sbase + ChunkSmem::RAW + i * kTile,
-                                sbase + ChunkSmem::K + i * kTile);
+      ah[i] = Rows{0, 0};
+      if (b0 + i < b1) ah[i] = load_rows<FP8, false>(a, a.p.v, a.p.k, pages[i], g, key0 + (b0 + i) * kBK, own0 + i * kTile, 2048);
       asm volatile("cp.async.commit_group;" ::: "memory");
     }
-    fetch_scales(ah[0]);
+    byte0 = fetch_scale(a.p.vs, ah[0]);
+    byte1 = fetch_scale(a.p.vs, ah[1]);
+    kbyte0 = fetch_scale(a.p.ks, ah[0]);
+    kbyte1 = fetch_scale(a.p.ks, ah[1]);
     int raw_slot = 0;
     for (int j = b0; j < b1; ++j) {
       const int n = j - b0, st = n % kST;
-      const uint32_t scale_bytes = next_k | (next_v << 8);
-      const uint32_t raw = sbase + ChunkSmem::RAW + raw_slot * kTile;
-      const uint32_t own = raw + (32 * w + lane) * 16;
-      const uint32_t ktile = sbase + ChunkSmem::K + st * kTile, vtile = sbase + ChunkSmem::V + st * kTile;
+      const uint32_t byte = byte0, kbyte = kbyte0;
+      byte0 = byte1;
+      kbyte0 = kbyte1;
+      const uint32_t own = own0 + raw_slot * kTile, vtile = sbase + ChunkSmem::V + st * kTile;
       asm volatile("cp.async.wait_group %0;" ::"n"(kRaw - 1) : "memory");
       const int k0 = lo + j * kBK;
-      const uint32_t there = ah[0].there;
       const bool partial = k0 < full_lo || k0 + kBK > full_hi;
       uint32_t broken = 0;  // keys of this warp
-      uint4 v[FP8 ? 4 : 8];
+      uint4 v[kPieces];
 #pragma unroll
-      for (int i = 0; i < (FP8 ? 4 : 8); ++i) v[i] = lds4(own + ((FP8 ? 4 : 0) + i) * 2048);
-      // ---- exponents of this block: largest K, largest V, smallest nonzero of each
-      uint32_t kmax = 0, vmax = 0, kmin = 255, vmin = 255;
+      for (int i = 0; i < kPieces; ++i) v[i] = lds4(own + i * 2048);
+      // ---- largest exponent of the block, and the smallest that is not of zeros: of a row (e4m3),
+      // of 8 values of a row (bf16)
+      uint32_t vmax = 0, vmin = 255;
       if constexpr (FP8) {
         if (partial) {
-          bool bad[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             uint32_t* x = reinterpret_cast<uint32_t*>(&v[i]);
-            bad[i] = false;
+            bool bad = false;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const uint32_t m = __vcmpeq4(x[e] & 0x7f7f7f7fu, 0x7f7f7f7fu);
-              bad[i] |= m != 0;
+              bad |= m != 0;
               x[e] &= ~m;
             }
-            uint32_t q = __ballot_sync(0xffffffffu, bad[i]);  // lanes 4 r .. 4 r + 3: key 8 i + r
-            q |= q >> 1;
-            q |= q >> 2;
-            q &= 0x11111111u;
+            const uint32_t q = any_of_groups(__ballot_sync(0xffffffffu, bad), 4);  // bit 4 r: key 8 i + r
 #pragma unroll
             for (int r = 0; r < 8; ++r) broken |= ((q >> (4 * r)) & 1u) << (8 * i + r);
           }
         }
-        uint32_t kb = scale_bytes & 255u, vb = (scale_bytes >> 8) & 255u;
-        if (kb == 255u) kb = 0;
-        if (((broken >> lane) & 1u) || vb == 255u) vb = 0;
-        kmax = __reduce_max_sync(0xffffffffu, kb);
-        vmax = __reduce_max_sync(0xffffffffu, vb);
-        kmin = __reduce_min_sync(0xffffffffu, kb ? kb : 255u);
-        vmin = __reduce_min_sync(0xffffffffu, vb ? vb : 255u);
+        const uint32_t vb = ((broken >> lane) & 1u) || byte == 255u ? 0u : byte;
+        vmax = vb;
+        vmin = vb ? vb : 255u;
       } else {
-        uint32_t all = 0, least = 255;
+        uint32_t all = 0, least = 0xffffu;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          uint32_t* x = reinterpret_cast<uint32_t*>(&v[i]);
-          uint32_t m2 = __vmaxu2(__vmaxu2(x[0] & 0x7fff7fffu, x[1] & 0x7fff7fffu),
-                                 __vmaxu2(x[2] & 0x7fff7fffu, x[3] & 0x7fff7fffu));
-          uint32_t m = max(m2 & 0xffffu, m2 >> 16);
-          if (__any_sync(0xffffffffu, m >= 0x7f80u)) {  // something is not finite
-            m = 0;
+          const uint32_t m2 = __vmaxu2(__vmaxu2(v[i].x & 0x7fff7fffu, v[i].y & 0x7fff7fffu),
+                                       __vmaxu2(v[i].z & 0x7fff7fffu, v[i].w & 0x7fff7fffu));
+          const uint32_t m = max(m2 & 0xffffu, m2 >> 16);
+          all = max(all, m);
+          least = min(least, m - 1u);  // 0 wraps to the largest
+        }
+        if (__any_sync(0xffffffffu, all >= 0x7f80u)) {  // something is not finite
+          all = 0;
+          least = 0xffffu;
+#pragma unroll 1
+          for (int i = 0; i < 8; ++i) {
+            const uint4 raw = lds4(own + i * 2048);
+            const uint32_t x[4] = {raw.x, raw.y, raw.z, raw.w};
+            uint32_t m = 0;
             bool bad = false;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -422,47 +419,67 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
               const uint32_t fin = x[e] & ~f & 0x7fff7fffu;
               m = max(m, max(fin & 0xffffu, fin >> 16));
               bad |= f != 0;
-              if (partial) x[e] &= ~f;
             }
-            uint32_t q = __ballot_sync(0xffffffffu, bad && partial);  // lanes 8 r .. 8 r + 7: key 4 i + r
+            if (bad && partial) {
+              const uint32_t y[4] = {x[0] & ~__vcmpeq2(x[0] & 0x7f807f80u, 0x7f807f80u), x[1] & ~__vcmpeq2(x[1] & 0x7f807f80u, 0x7f807f80u),
+                                     x[2] & ~__vcmpeq2(x[2] & 0x7f807f80u, 0x7f807f80u), x[3] & ~__vcmpeq2(x[3] & 0x7f807f80u, 0x7f807f80u)};
+              st4(own + i * 2048, y[0], y[1], y[2], y[3]);
+            }
+            const uint32_t q = any_of_groups(__ballot_sync(0xffffffffu, bad && partial), 8);  // bit 8 r: key 4 i + r
 #pragma unroll
-            for (int r = 0; r < 4; ++r) broken |= (((q >> (8 * r)) & 255u) ? 1u : 0u) << (4 * i + r);
+            for (int r = 0; r < 4; ++r) broken |= ((q >> (8 * r)) & 1u) << (4 * i + r);
+            all = max(all, m);
+            least = min(least, m - 1u);
           }
-          m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-          m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-          m = max(m, __shfl_xor_sync(0xffffffffu, m, 4));
-          all = max(all, m >> 7);
-          if (m >> 7) least = min(least, m >> 7);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] = lds4(own + i * 2048);
         }
-        vmax = __reduce_max_sync(0xffffffffu, all);
-        vmin = __reduce_min_sync(0xffffffffu, least);
+        vmax = all >> 7;
+        vmin = least >= 0xffffu ? 255u : (least + 1u) >> 7;
       }
-      if (lane == 0) b->red[n & 1][w][0] = kmax | (vmax << 8) | (kmin << 16) | (vmin << 24);
+      vmax = __reduce_max_sync(0xffffffffu, vmax);
+      vmin = __reduce_min_sync(0xffffffffu, vmin);
+      uint32_t kmax = 0, kmin = 255;
+      if constexpr (FP8) {
+        const uint32_t kb = kbyte == 255u ? 0u : kbyte;
+        kmax = __reduce_max_sync(0xffffffffu, kb);
+        kmin = __reduce_min_sync(0xffffffffu, kb ? kb : 255u);
+      }
+      if (lane == 0) b->red[n & 1][w] = vmax | (vmin << 8) | (kmax << 16) | (kmin << 24);
       named_barrier_sync(1, 128);
-      uint32_t kt = 0, vt = 0, kl = 255, vl = 255;
+      uint32_t most = 0, least = 255;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint32_t x = b->red[n & 1][i][0];
-        kt = max(kt, x & 255u);
-        vt = max(vt, (x >> 8) & 255u);
-        kl = min(kl, (x >> 16) & 255u);
-        vl = min(vl, x >> 24);
+        const uint32_t x = b->red[n & 1][i];
+        most = max(most, x & 255u);
+        least = min(least, (x >> 8) & 255u);
+        kmax = max(kmax, (x >> 16) & 255u);
+        kmin = min(kmin, x >> 24);
       }
-      top = max(top, vt);
-      if (threadIdx.x == 0 && ((kl != 255u && kt - kl > (uint32_t)kWideRange) || (vl != 255u && (int)(top - vl) > kWideRange)))
-        b->wide = 1;
+      top = max(top, most);
+      if (threadIdx.x == 0) {
+        if (least != 255u && (int)(top - least) > (FP8 ? kWideRange : kWideRangeBf16)) b->wide = 1;
+        if (FP8 && kmin != 255u && (int)(kmax - kmin) > kWideRange) b->wide = 1;
+      }
       if (!dead && n >= kST && !mbar_wait(&b->kv_empty[st], ((n / kST) & 1) ^ 1, err, &b->abort_flag)) dead = true;
-      // ---- expand into the f16 tiles
+      // ---- expand into the f16 tile
       if constexpr (FP8) {
-        const int c = lane & 3;
+        // (each key's lane works out its factor, and all of them travel before the first store: left
+        // to the loop below, the stores kept the rows one after the other)
+        const uint32_t mine = h2_pow2(min((int)byte - (int)top, 0));
+        uint32_t mul[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = 8 * i + (lane >> 2);
-          const uint32_t sc = __shfl_sync(0xffffffffu, scale_bytes, r);
-          const uint4 k = lds4(own + i * 2048);
-          expand16(ktile, 32 * w + r, c, k, h2_pow2(min((int)(sc & 255u) - (int)kt, 0)));
-          expand16(vtile, 32 * w + r, c, v[i], h2_pow2(min((int)((sc >> 8) & 255u) - (int)top, 0)));
-        }
+        for (int i = 0; i < 4; ++i) mul[i] = __shfl_sync(0xffffffffu, mine, 8 * i + (lane >> 2));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) expand16(vtile, 32 * w + 8 * i + (lane >> 2), lane & 3, v[i], mul[i]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = lds4(own + (4 + i) * 2048);
+        const uint32_t kmine = h2_pow2(min((int)kbyte - (int)kmax, 0));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mul[i] = __shfl_sync(0xffffffffu, kmine, 8 * i + (lane >> 2));
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          expand16(sbase + ChunkSmem::K + st * kTile, 32 * w + 8 * i + (lane >> 2), lane & 3, v[i], mul[i]);
       } else {
         // largest |V'| in [2^8, 2^9): v * 2^(135 - top)
         const float f = pow2i(135 - (int)max(top, 9u));
@@ -482,35 +499,67 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
         }
       }
       if (lane == 0) {
-        b->info[st].there[w] = there;
+        b->info[st].there[w] = ah[0].there;
         b->info[st].broken[w] = broken;
       }
-      if (threadIdx.x == 0) {
-        b->info[st].kmul = FP8 ? pow2i((int)kt - 127) : 1.f;
-        b->info[st].unit = FP8 ? (int)top - 127 : (int)max(top, 9u) - 135;
-      }
+      if (threadIdx.x == 0) b->info[st].kmul = FP8 ? pow2i((int)kmax - 127) : 1.f;
+      if (threadIdx.x == 0) b->info[st].unit = FP8 ? (int)top - 127 : (int)max(top, 9u) - 135;
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&b->kv_full[st]);
       // ---- refill
 #pragma unroll
       for (int i = 0; i < kRaw - 1; ++i) ah[i] = ah[i + 1];
-      ah[kRaw - 1].there = 0;
+      ah[kRaw - 1] = Rows{0, 0};
       if (j + kRaw < b1) {
-        const int ns = (n + kRaw) % kST;
-        if (!FP8 && !dead && n + kRaw >= kST &&   // K goes straight into its tile
-            !mbar_wait(&b->kv_empty[ns], (((n + kRaw) / kST) & 1) ^ 1, err, &b->abort_flag))
-          dead = true;
         const int page = next_page;
-        if (j + kRaw + 1 < b1) next_page = page_of(a, table, lane_key + (j + kRaw + 1) * kBK, hi);
-        ah[kRaw - 1] = load_block<FP8>(a, page, g, lo + (j + kRaw) * kBK, w, lane, raw, sbase + ChunkSmem::K + ns * kTile);
+        if (j + kRaw + 1 < b1) next_page = page_of(a, table, key0 + lane + (j + kRaw + 1) * kBK, hi);
+        ah[kRaw - 1] = load_rows<FP8, false>(a, a.p.v, a.p.k, page, g, key0 + (j + kRaw) * kBK, own, 2048);
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
-      fetch_scales(ah[0]);
+      byte1 = fetch_scale(a.p.vs, ah[1]);
+      kbyte1 = fetch_scale(a.p.ks, ah[1]);
       raw_slot = raw_slot + 1 == kRaw ? 0 : raw_slot + 1;
     }
   } else if (warp >= 12) {
-    setmaxnreg_dec<40>();
+    setmaxnreg_dec<72>();
+    if (!FP8 && warp >= 14) {  // bf16 K: 64 keys a warp, in two groups of 32, straight into their tile
+      const int w = warp - 14;
+      bool dead = false;
+      const int key0 = lo + 64 * w + lane;
+      int next_page[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) next_page[u] = b0 < b1 ? page_of(a, table, key0 + 32 * u + b0 * kBK, hi) : -1;
+      auto load = [&](int j) {
+        const int page[2] = {next_page[0], next_page[1]};
+        if (j + 1 < b1) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u) next_page[u] = page_of(a, table, key0 + 32 * u + (j + 1) * kBK, hi);
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          load_rows<FP8, true>(a, a.p.k, nullptr, page[u], g, lo + 64 * w + 32 * u + j * kBK,
+                               sbase + ChunkSmem::K + ((j - b0) % kST) * kTile, 64 * w + 32 * u);
+      };
+#pragma unroll 1
+      for (int i = 0; i < kRaw; ++i) {
+        if (b0 + i < b1) load(b0 + i);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      }
+#pragma unroll 1
+      for (int j = b0; j < b1; ++j) {
+        const int n = j - b0, m = n + kRaw;
+        asm volatile("cp.async.wait_group %0;" ::"n"(kRaw - 1) : "memory");
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&b->kv_full[n % kST]);
+        if (j + kRaw < b1) {
+          if (!dead && m >= kST && !mbar_wait(&b->kv_empty[m % kST], ((m / kST) & 1) ^ 1, err, &b->abort_flag)) dead = true;
+          load(j + kRaw);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      }
+    }
     if (warp == 12 && b1 > b0 && elect_one_sync()) {
       const uint32_t sqa = sbase + ChunkSmem::Q, sk0 = sbase + ChunkSmem::K, sv0 = sbase + ChunkSmem::V;
       Issue ta{tl[0].jlo, tl[0].jhi, 0, 0}, tb{tl[1].jlo, tl[1].jhi, 0, 0};
@@ -528,7 +577,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
       }
     }
   } else {
-    setmaxnreg_inc<192>();
+    setmaxnreg_inc<184>();
     const int x = (warp - 4) >> 2;
     const Tile t = x ? tl[1] : tl[0];
     const int row = (warp & 3) * 32 + lane;
@@ -637,7 +686,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
       const float mraw = fmax3(fmax3(mxp[0], mxp[1], mxp[2]), fmax3(mxp[3], mxp[4], mxp[5]), fmaxf(mxp[6], mxp[7]));
       const float cand = mraw == -INFINITY ? -INFINITY : mraw * smul - kTopLog2;
       float alpha = 1.f;
-      bool resc = cand > m_ref + kGrowLog2;
+      bool resc = cand > m_ref;
       if (resc) {
         alpha = ex2a(m_ref - cand);
         m_ref = cand;
