@@ -71,8 +71,8 @@ void paged_attention(torch::Tensor q, torch::Tensor k_pages, torch::Tensor v_pag
   auto stream = at::cuda::getCurrentCUDAStream();
   max_q_len = std::max<int64_t>(max_q_len, 1);
   max_seq_len = std::max<int64_t>(max_seq_len, 1);
-  if (std::min<int64_t>(max_q_len, a.T) * a.group <= kFewRows)
-    launch_few(a, max_q_len, max_seq_len, stream);
+  if (a.group <= kFewRows && std::min<int64_t>(max_q_len, a.T) * a.group <= kFewTotal)
+    launch_few(a, std::min<int64_t>(max_q_len, a.T), max_seq_len, stream);
   else
     launch_chunk(a, max_q_len, max_seq_len, stream);
 }

@@ -5,7 +5,12 @@
 namespace af3 {
 namespace paged {
 
-constexpr int kFewRows = 32;  // query rows a KV head that launch_few takes in one tile
+constexpr int kFewRows = 32;  // query rows a KV head of launch_few's largest tile: its largest group
+
+// Sequences of up to this many query rows a KV head go to launch_few.  Measured on 4200 tokens, 8
+// heads a KV head, e4m3, launch_few against launch_chunk: 64 sequences of 4 tokens (32 rows) 198 and
+// 286 us, of 5 (40 rows) 259 and 253 us, of 8 (64 rows) 320 and 253 us; 8 sequences of 5: 44 and 58 us.
+constexpr int kFewTotal = 40;
 
 // Where the V (or K) scale bytes of keys that share a tile are further apart than this many
 // powers of two, f16 no longer holds all of them well enough once a row does not see the largest;
@@ -14,7 +19,7 @@ constexpr int kWideRange = 14;
 // bf16 V scaled to f16 keeps 2^-25 of 2^8; judged by 8 values at a time.
 constexpr int kWideRangeBf16 = 18;
 
-// At most kFewRows query rows a KV head and sequence: memory-bound, split over the keys.
+// Few query rows a KV head and sequence, groups of at most kFewRows: memory-bound, split over the keys.
 void launch_few(const Args& a, int64_t max_q, int64_t max_len, cudaStream_t stream);
 
 // Any number of rows, at most 128 query heads a KV head: tensor cores, split over the keys when

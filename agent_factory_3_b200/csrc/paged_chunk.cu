@@ -336,8 +336,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
     uint32_t top = 0;  // largest e8m0 byte (e4m3) or biased exponent (bf16) so far
     bool dead = false;
     Rows ah[kRaw];
-    // scale bytes of the next two blocks, loaded two blocks before they are used
-    uint32_t byte0 = 0, byte1 = 0, kbyte0 = 0, kbyte1 = 0;
+    // Scale bytes of the block to expand.  Those of the next block are asked for at the top of a round
+    // and moved here at its end: a move right after the load would wait for it (1000 cycles a block).
+    uint32_t byte = 0, kbyte = 0;
     auto fetch_scale = [&](const uint8_t* from, const Rows& h) -> uint32_t {
       return FP8 ? load_byte(from + h.scale, (h.there >> lane) & 1u) : 0u;
     };
@@ -353,16 +354,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
       if (b0 + i < b1) ah[i] = load_rows<FP8, false>(a, a.p.v, a.p.k, pages[i], g, key0 + (b0 + i) * kBK, own0 + i * kTile, 2048);
       asm volatile("cp.async.commit_group;" ::: "memory");
     }
-    byte0 = fetch_scale(a.p.vs, ah[0]);
-    byte1 = fetch_scale(a.p.vs, ah[1]);
-    kbyte0 = fetch_scale(a.p.ks, ah[0]);
-    kbyte1 = fetch_scale(a.p.ks, ah[1]);
+    byte = fetch_scale(a.p.vs, ah[0]);
+    kbyte = fetch_scale(a.p.ks, ah[0]);
     int raw_slot = 0;
     for (int j = b0; j < b1; ++j) {
       const int n = j - b0, st = n % kST;
-      const uint32_t byte = byte0, kbyte = kbyte0;
-      byte0 = byte1;
-      kbyte0 = kbyte1;
+      const uint32_t next_byte = fetch_scale(a.p.vs, ah[1]), next_kbyte = fetch_scale(a.p.ks, ah[1]);
       const uint32_t own = own0 + raw_slot * kTile, vtile = sbase + ChunkSmem::V + st * kTile;
       asm volatile("cp.async.wait_group %0;" ::"n"(kRaw - 1) : "memory");
       const int k0 = lo + j * kBK;
@@ -517,8 +514,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
         ah[kRaw - 1] = load_rows<FP8, false>(a, a.p.v, a.p.k, page, g, key0 + (j + kRaw) * kBK, own, 2048);
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
-      byte1 = fetch_scale(a.p.vs, ah[1]);
-      kbyte1 = fetch_scale(a.p.ks, ah[1]);
+      byte = next_byte;
+      kbyte = next_kbyte;
       raw_slot = raw_slot + 1 == kRaw ? 0 : raw_slot + 1;
     }
   } else if (warp >= 12) {

@@ -36,6 +36,8 @@ namespace cg = cooperative_groups;
 namespace af3 {
 namespace paged {
 
+constexpr int kMaxSplits = 8;  // the largest portable cluster
+
 // Two shapes of CTA.  Long: 8 warps, 3 blocks in flight each.  Short (a part of at most 8 blocks:
 // short contexts, sliding windows): 4 warps with 2 blocks each, all of them on their way at once, and
 // small enough that several CTAs share an SM.
@@ -236,7 +238,7 @@ __device__ __forceinline__ Keys issue_block(const Args& a, const uint8_t* kb, co
 
 template <bool FP8, int NT, bool LONG, bool ONE>
 __global__ void __launch_bounds__(FewCfg<FP8, NT, LONG>::kThreads, FewCfg<FP8, NT, LONG>::kBlocksPerSm)
-    paged_few_kernel(const Args a, const int rows_per_tile, const int splits) {
+    paged_few_kernel(const Args a, const int rows_per_tile, const int tiles, const int splits) {
   using C = FewCfg<FP8, NT, LONG>;
   constexpr int kWarps = C::kWarps, kStages = C::kStages;
   constexpr int R = NT * 8;  // query rows of a tile
@@ -248,7 +250,7 @@ __global__ void __launch_bounds__(FewCfg<FP8, NT, LONG>::kThreads, FewCfg<FP8, N
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int grp = lane >> 2, tig = lane & 3;
   const int rank = splits > 1 ? (int)blockIdx.x : 0;
-  const int g = blockIdx.y, b = blockIdx.z;
+  const int g = blockIdx.y / tiles, b = blockIdx.z;
   const Seq sq = load_seq(a, b);
   const int tokens_per_tile = rows_per_tile / a.group;
   const int* table = a.table + (int64_t)b * a.ld_table;
@@ -259,7 +261,8 @@ __global__ void __launch_bounds__(FewCfg<FP8, NT, LONG>::kThreads, FewCfg<FP8, N
   const int64_t byte = (int64_t)g * a.p.s_head + lane * a.p.s_token;
   const uint8_t *kb0 = a.p.k + piece, *vb0 = a.p.v + piece, *ksb = a.p.ks + byte, *vsb = a.p.vs + byte;
 
-  for (int tok0 = sq.t0; tok0 < sq.t1; tok0 += tokens_per_tile) {
+  // (one round when the caller's longest q is right)
+  for (int tok0 = sq.t0 + (int)(blockIdx.y % tiles) * tokens_per_tile; tok0 < sq.t1; tok0 += tiles * tokens_per_tile) {
     const int ntok = min(tokens_per_tile, sq.t1 - tok0);
     const int nrows = ntok * a.group;
     const bool several = ntok > 1;  // rows differ in what they see
@@ -675,13 +678,20 @@ __global__ void __launch_bounds__(FewCfg<FP8, NT, LONG>::kThreads, FewCfg<FP8, N
       for (int x = 16; x > 0; x >>= 1) den += __shfl_xor_sync(0xffffffffu, den, x);
       den += ex2a(sk - tu);
       float x = 0.f, y = 0.f;
-      for (int c = 0; c < splits; ++c) {
+      const float2* mine = reinterpret_cast<const float2*>(c_o) + r * (kD / 2) + lane;
+      float2 v[kMaxSplits];  // every CTA's part is asked for before the first is used
+#pragma unroll
+      for (int c = 0; c < kMaxSplits; ++c) {
+        v[c] = make_float2(0.f, 0.f);
+        if (c < splits) v[c] = splits > 1 ? *cg::this_cluster().map_shared_rank(mine, c) : *mine;
+      }
+#pragma unroll
+      for (int c = 0; c < kMaxSplits; ++c) {
         const float fc = __shfl_sync(0xffffffffu, f, c);
-        const float2* src = reinterpret_cast<const float2*>(c_o) + r * (kD / 2) + lane;
-        if (splits > 1) src = cg::this_cluster().map_shared_rank(src, c);
-        const float2 v = *src;
-        x = fmaf(fc, v.x, x);
-        y = fmaf(fc, v.y, y);
+        if (c < splits) {
+          x = fmaf(fc, v[c].x, x);
+          y = fmaf(fc, v[c].y, y);
+        }
       }
       const float inv = den == 0.f ? 0.f : 1.f / den;
       x *= inv;
@@ -711,12 +721,11 @@ static int clusters_at_once(K kern, const cudaLaunchConfig_t& cfg) {
 }
 
 template <bool FP8, int NT, bool LONG, bool ONE>
-static void launch_few_nt(const Args& a, int rows_per_tile, int64_t keys, cudaStream_t stream) {
+static void launch_few_nt(const Args& a, int rows_per_tile, int max_q, int64_t keys, cudaStream_t stream) {
   using C = FewCfg<FP8, NT, LONG>;
   constexpr int smem = C::kWarps * C::kRingBytes + NT * 8 * kD * 4;
   static_assert(NT * 8 * kD * 4 <= C::kRingBytes, "a warp's part has to fit its ring");
   auto kern = paged_few_kernel<FP8, NT, LONG, ONE>;
-  constexpr int kMaxSplits = 8;  // the largest portable cluster
   static int at_once[64][kMaxSplits + 1] = {};
   int dev;
   AF3_CUDA_CHECK(cudaGetDevice(&dev));
@@ -739,7 +748,8 @@ static void launch_few_nt(const Args& a, int rows_per_tile, int64_t keys, cudaSt
   // The keys are split so that the number of rounds of clusters times the length of one is least:
   // a CTA takes as long as kFixed keys to begin and to end (5 us against some 150 keys a us), and
   // half a round is lost at the end when there are several.
-  const int64_t items = (int64_t)a.B * a.hkv;
+  const int tokens = rows_per_tile / a.group, tiles = (max_q + tokens - 1) / tokens;
+  const int64_t items = (int64_t)a.B * a.hkv * tiles;
   constexpr double kFixed = 768;
   int splits = 1;
   double best = 0;
@@ -751,26 +761,30 @@ static void launch_few_nt(const Args& a, int rows_per_tile, int64_t keys, cudaSt
       splits = s;
     }
   }
-  cfg.gridDim = dim3((unsigned)splits, (unsigned)a.hkv, (unsigned)a.B);
+  cfg.gridDim = dim3((unsigned)splits, (unsigned)(a.hkv * tiles), (unsigned)a.B);
   attr[0].val.clusterDim = {(unsigned)splits, 1, 1};
   cfg.numAttrs = splits > 1 ? 1 : 0;
-  AF3_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, a, rows_per_tile, splits));
+  AF3_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, a, rows_per_tile, tiles, splits));
 }
 
 template <bool FP8, bool LONG, bool ONE>
 static void launch_few_t(const Args& a, int max_q, int64_t keys, cudaStream_t stream) {
-  const int want = std::max(std::min(max_q, kFewRows / a.group), 1) * a.group;  // rows of a tile
+  // Up to 16 rows in one tile.  More rows take tiles of 16 that read the keys side by side, from L2
+  // but for one of them: 64 sequences of 5 tokens (40 rows) take 120 us so, 132 us in tiles of 32,
+  // whose registers leave half the warps.  A group of more than 16 heads needs the larger tile.
+  const int rows = a.group > 16 ? kFewRows : 16;
+  const int want = std::max(std::min(max_q, rows / a.group), 1) * a.group;  // rows of a tile
   if (want <= 8)
-    launch_few_nt<FP8, 1, LONG, ONE>(a, want, keys, stream);
+    launch_few_nt<FP8, 1, LONG, ONE>(a, want, max_q, keys, stream);
   else if (want <= 16)
-    launch_few_nt<FP8, 2, LONG, ONE>(a, want, keys, stream);
+    launch_few_nt<FP8, 2, LONG, ONE>(a, want, max_q, keys, stream);
   else
-    launch_few_nt<FP8, 4, LONG, ONE>(a, want, keys, stream);
+    launch_few_nt<FP8, 4, LONG, ONE>(a, want, max_q, keys, stream);
 }
 
 void launch_few(const Args& a, int64_t max_q, int64_t max_len, cudaStream_t stream) {
   const int64_t keys = a.window > 0 ? std::min<int64_t>(max_len, a.window + max_q) : max_len;
-  const int q = (int)std::min<int64_t>(max_q, kFewRows);
+  const int q = (int)std::min<int64_t>(max_q, kFewTotal);
   // 8 blocks of 32 keys for 4 warps; a part of more in the short shape only runs slower
   const bool is_long = keys > 256 && (keys > 8 * 256 || (int64_t)a.B * a.hkv * 8 > 3 * (int64_t)num_sms());
   const bool one = (a.p.page_size & 31) == 0;

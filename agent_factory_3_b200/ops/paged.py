@@ -109,8 +109,9 @@ def kv_store_fp8(qkv, k_off, v_off, slots, k_pages, v_pages, k_scales, v_scales)
     pool (e.g. -1) is skipped."""
     if not use_cuda_kernels(qkv):
         return kv_store_fp8_reference(qkv, k_off, v_off, slots, k_pages, v_pages, k_scales, v_scales)
-    ext().kv_store_fp8(qkv, k_off, v_off, slots.to(torch.int32).contiguous(), k_pages, v_pages,
-                       k_scales, v_scales)
+    if slots.dtype != torch.int32 or not slots.is_contiguous():
+        slots = slots.to(torch.int32).contiguous()
+    ext().kv_store_fp8(qkv, k_off, v_off, slots, k_pages, v_pages, k_scales, v_scales)
 
 
 def kv_gather_fp8(qkv, k_off, v_off, slots, k_pages, v_pages, k_scales, v_scales) -> None:
@@ -118,8 +119,9 @@ def kv_gather_fp8(qkv, k_off, v_off, slots, k_pages, v_pages, k_scales, v_scales
     Rows of slots outside the pool keep what they hold."""
     if not use_cuda_kernels(qkv):
         return kv_gather_fp8_reference(qkv, k_off, v_off, slots, k_pages, v_pages, k_scales, v_scales)
-    ext().kv_gather_fp8(qkv, k_off, v_off, slots.to(torch.int32).contiguous(), k_pages, v_pages,
-                        k_scales, v_scales)
+    if slots.dtype != torch.int32 or not slots.is_contiguous():
+        slots = slots.to(torch.int32).contiguous()
+    ext().kv_gather_fp8(qkv, k_off, v_off, slots, k_pages, v_pages, k_scales, v_scales)
 
 
 def paged_attention_reference(q, k_pages, v_pages, page_table, seq_lens, cu_q, sinks, hq, hkv,
