@@ -66,7 +66,7 @@ void paged_attention(torch::Tensor q, torch::Tensor k_pages, torch::Tensor v_pag
   a.hq = (int)hq;
   a.hkv = (int)hkv;
   a.group = (int)(hq / hkv);
-  a.window = (int)window;
+  a.window = (int)std::min<int64_t>(window, int64_t(1) << 30);  // (differences of positions stay in 32 bits)
   a.scale_log2 = (float)scale * kLog2e;
   auto stream = at::cuda::getCurrentCUDAStream();
   max_q_len = std::max<int64_t>(max_q_len, 1);

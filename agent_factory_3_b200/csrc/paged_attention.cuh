@@ -44,7 +44,7 @@ __device__ __forceinline__ Seq load_seq(const Args& a, int b) {
   Seq s;
   s.t0 = min(max(a.cu[b], 0), a.T);
   s.t1 = min(max(a.cu[b + 1], s.t0), a.T);
-  const int len = max(a.lens[b], 0);
+  const int len = min(max(a.lens[b], 0), 1 << 30);
   s.first = len - (s.t1 - s.t0);
   const int64_t cap = (int64_t)a.max_pages * a.p.page_size;
   s.key_end = (int)min((int64_t)len, cap);

@@ -106,7 +106,7 @@ def kv_gather_fp8_reference(qkv, k_off, v_off, slots, k_pages, v_pages, k_scales
 def kv_store_fp8(qkv, k_off, v_off, slots, k_pages, v_pages, k_scales, v_scales) -> None:
     """K/V of row i of qkv [n, width] (Hkv * D values from columns k_off and v_off) -> page slot
     slots[i] (slot = page * page_size + offset) as e4m3 codes and scale bytes.  A slot outside the
-    pool (e.g. -1) is skipped."""
+    pool (e.g. -1) is skipped; the others must be distinct."""
     if not use_cuda_kernels(qkv):
         return kv_store_fp8_reference(qkv, k_off, v_off, slots, k_pages, v_pages, k_scales, v_scales)
     if slots.dtype != torch.int32 or not slots.is_contiguous():
