@@ -61,8 +61,8 @@ struct ChunkSmem {
 };
 
 struct StageInfo {
-  uint32_t there[4];   // keys that exist and lie in the span's range
-  uint32_t broken[4];  // keys whose V is not finite (cleared), in blocks not seen by every row
+  uint32_t there[4];   // keys that exist and lie in the span's range, but for the broken ones
+  uint32_t broken[4];  // those whose V is not finite (cleared), in blocks not seen by every row
   float kmul;          // 2^ek (e4m3)
   int unit;            // V' is in units of 2^unit
 };
@@ -502,7 +502,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
         }
       }
       if (lane == 0) {
-        b->info[st].there[w] = ah[0].there;
+        b->info[st].there[w] = ah[0].there & ~broken;
         b->info[st].broken[w] = broken;
       }
       if (threadIdx.x == 0) b->info[st].kmul = FP8 ? pow2i((int)kmax - 127) : 1.f;
@@ -658,6 +658,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
       const int new_unit = info->unit;
       const int k0 = j * kBK;  // relative to lo
       const uint32_t all4 = info->there[0] & info->there[1] & info->there[2] & info->there[3];
+      // (a broken key is not in `there`: a tile may see all of a block that the span does not)
       const bool need_mask = k0 < tile_lo || k0 + kBK > tile_hi || all4 != 0xffffffffu;
       if (need_mask) {
         uint32_t hit = 0;
@@ -665,7 +666,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
         for (int w = 0; w < 4; ++w) {
           // bits of keys k0 + 32 w + e in [see_lo, see_hi)
           const int f = min(max(see_lo - (k0 + 32 * w), 0), 32), e1 = min(max(see_hi - (k0 + 32 * w), 0), 32);
-          uint32_t vis = info->there[w];
+          uint32_t vis = info->there[w] | info->broken[w];
           vis &= f >= 32 ? 0u : 0xffffffffu << f;
           vis &= e1 >= 32 ? 0xffffffffu : (1u << e1) - 1u;
           hit |= vis & info->broken[w];

@@ -1,0 +1,64 @@
+"""Attention over cache pages where values differ in magnitude or are not finite, on the GPU
+against 64 bits.  Tolerance: that of test_paged_gpu.check, a bf16 rounding of the output and
+2^-12 of A, the same attention over |V|."""
+import math
+
+import pytest
+import torch
+
+from test_paged_gpu import check, make
+
+from agent_factory_3_b200.ops import paged
+
+pytestmark = pytest.mark.gpu
+
+
+def slots_of(a, page):
+    """Slots of the keys of sequence 0, in order."""
+    n = int(a["seq_lens"][0])
+    t = a["page_table"][0].long()
+    j = torch.arange(n, device=t.device)
+    return t[j // page] * page + j % page
+
+
+def put(a, page, keys, k=None, v=None):
+    """Writes rows [len(keys), Hkv, 64] into the pages at these keys of sequence 0."""
+    at = slots_of(a, page)[torch.as_tensor(keys, device=a["q"].device)]
+    hkv = a["hkv"]
+    old = [paged.dequantize_rows_reference(
+        p.view(torch.uint8)[at // page, at % page].view(paged.FP8), s[at // page, :, at % page])
+        if s is not None else p[at // page, at % page].float()
+        for p, s in ((a["k_pages"], a["k_scales"]), (a["v_pages"], a["v_scales"]))]
+    k, v = (old[i] if x is None else x.float().expand(at.numel(), hkv, 64) for i, x in ((0, k), (1, v)))
+    if a["k_scales"] is None:
+        a["k_pages"][at // page, at % page] = k.bfloat16()
+        a["v_pages"][at // page, at % page] = v.bfloat16()
+    else:
+        rows = torch.cat([k.reshape(-1, hkv * 64), v.reshape(-1, hkv * 64)], 1).bfloat16()
+        paged.kv_store_fp8(rows, 0, hkv * 64, at.to(torch.int32), a["k_pages"], a["v_pages"],
+                           a["k_scales"], a["v_scales"])
+
+
+# ------------------------------------------------------------- values that are not finite
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("q,start,hq,hkv,window,key", [
+    (256, 0, 2, 2, 0, 5),          # one head a KV head: rows 128 .. 255 see all of block 0
+    (32, 112, 16, 2, 0, 5),        # tokens 16 .. 31 see all of block 0, tokens 0 .. 15 do not
+    (32, 112, 16, 2, 0, 120),
+    (40, 230, 64, 8, 0, 255),
+    (2, 300, 128, 1, 200, 101),    # block 0 is whole for the first token only
+    (2, 300, 128, 1, 200, 150),
+    (64, 600, 16, 2, 300, 500),
+])
+def test_broken_value_that_whole_tiles_see(dev, fp8, q, start, hq, hkv, window, key):
+    page = 16
+    a = make(dev, [q], [start + q], hq, hkv, page, fp8)
+    at = int(slots_of(a, page)[key])
+    if fp8:
+        a["v_pages"].view(torch.uint8)[at // page, at % page, :, 7] = 0x7F
+    else:
+        a["v_pages"][at // page, at % page, :, 7] = math.nan
+    out = check(a, window)
+    pos = start + torch.arange(q, device=dev)
+    sees = (pos >= key) & ((pos - key < window) if window else (pos >= 0))
+    assert torch.equal(torch.isnan(out.view(q, hq, 64)[..., 7]).all(1), sees)
