@@ -13,8 +13,9 @@ constexpr int kFewRows = 32;  // query rows a KV head of launch_few's largest ti
 constexpr int kFewTotal = 40;
 
 // Where the V (or K) scale bytes of keys that share a tile are further apart than this many
-// powers of two, f16 no longer holds all of them well enough once a row does not see the largest;
-// such a tile's rows are taken key by key.  Tokens of one sequence differ by far less.
+// powers of two, f16 no longer holds all of them well enough for a row in which the largest have little
+// weight or none; such a tile's rows are taken key by key.  At 14 the values at the small end still meet
+// weights of 2^-10 of the row's largest in 11 bits.  Tokens of one sequence differ by far less.
 constexpr int kWideRange = 14;
 // bf16 V scaled to f16 keeps 2^-25 of 2^8; judged by 8 values at a time.
 constexpr int kWideRangeBf16 = 18;

@@ -19,8 +19,10 @@
 //
 // e4m3 pages: codes are expanded to f16 (exact).  K's scale multiplies the score in fp32.  V's scale
 // is folded into P: P' = p * 2^(e - E) with E the largest V exponent seen by this warp so far; O is
-// rescaled when E grows.  The largest p is 2^10, so P' keeps f16's 11 bits down to 2^-24 of it.  The
-// query rows are brought to f16 after a power-of-two scaling to [1, 2), undone in fp32.
+// rescaled when E grows.  The largest p is 2^10, so P' keeps f16's 11 bits down to 2^-24 of it; rows
+// that met exponents more than kWideRange apart are taken key by key (the values of the largest may
+// have next to no weight).  The query rows are brought to f16 after a power-of-two scaling to [1, 2),
+// undone in fp32.
 // (An e4m3 code costs one conversion of half rate; integer conversions took three times as long.)
 // bf16 pages: K, V, Q as they are; P as the sum of two bf16 numbers (16 bits), since one alone would
 // cost as much precision as the rounding of the output.  The 8 more instructions of 32 keys hide
@@ -643,8 +645,8 @@ __global__ void __launch_bounds__(FewCfg<FP8, NT, LONG>::kThreads, FewCfg<FP8, N
     // ---- join the warps: one warp a row, lane l has dims 2l, 2l + 1
     bool wide = false;
     if constexpr (FP8) {
-      if (several)
-        for (int w = 0; w < kWarps; ++w) wide |= s_wide[w] != 0;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) wide |= s_wide[w] != 0;
     }
     for (int r = warp; r < nrows; r += kWarps) {
       float mm = -INFINITY;

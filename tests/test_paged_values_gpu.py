@@ -62,3 +62,23 @@ def test_broken_value_that_whole_tiles_see(dev, fp8, q, start, hq, hkv, window, 
     pos = start + torch.arange(q, device=dev)
     sees = (pos >= key) & ((pos - key < window) if window else (pos >= 0))
     assert torch.equal(torch.isnan(out.view(q, hq, 64)[..., 7]).all(1), sees)
+
+
+# ------------------------------------------------------------- magnitudes
+@pytest.mark.parametrize("span", [16, 28, 40, 60])
+@pytest.mark.parametrize("q,ctx,hq,hkv", [(1, 40, 16, 2), (1, 300, 8, 1), (1, 5000, 64, 8), (1, 700, 32, 1),
+                                          (3, 400, 8, 1), (60, 500, 16, 2)])
+def test_large_value_without_weight(dev, q, ctx, hq, hkv, span):
+    """e4m3: a token whose value is 2^span times the others' and whose weight is e^-100."""
+    page = 16
+    a = make(dev, [q], [ctx], hq, hkv, page, True)
+    u = torch.randn(64, device=dev).bfloat16()
+    a["q"] = u.repeat(q, hq).contiguous()
+    keys = torch.arange(ctx)
+    k = 0.05 * torch.randn(ctx, hkv, 64, device=dev)
+    v = torch.randn(ctx, hkv, 64, device=dev)
+    for at in (1, ctx // 2):
+        k[at] = -800.0 * u.float() / u.float().square().sum()      # scores of -100
+        v[at] *= 2.0 ** span
+    put(a, page, keys, k, v)
+    check(a)
