@@ -12,13 +12,11 @@ constexpr int kFewRows = 32;  // query rows a KV head of launch_few's largest ti
 // 286 us, of 5 (40 rows) 259 and 253 us, of 8 (64 rows) 320 and 253 us; 8 sequences of 5: 44 and 58 us.
 constexpr int kFewTotal = 40;
 
-// Where the V (or K) scale bytes of keys that share a tile are further apart than this many
+// e4m3 pages: where the V (or K) scale bytes of keys that share a tile are further apart than this many
 // powers of two, f16 no longer holds all of them well enough for a row in which the largest have little
 // weight or none; such a tile's rows are taken key by key.  At 14 the values at the small end still meet
 // weights of 2^-10 of the row's largest in 11 bits.  Tokens of one sequence differ by far less.
 constexpr int kWideRange = 14;
-// bf16 V scaled to f16 keeps 2^-25 of 2^8; judged by 8 values at a time.
-constexpr int kWideRangeBf16 = 18;
 
 // Few query rows a KV head and sequence, groups of at most kFewRows: memory-bound, split over the keys.
 void launch_few(const Args& a, int64_t max_q, int64_t max_len, cudaStream_t stream);

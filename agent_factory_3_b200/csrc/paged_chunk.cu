@@ -5,33 +5,36 @@
 // group) pair, floor(128 / group) tokens a tile, so the whole group shares every K/V block.  Few
 // spans over a long context are split: the CTAs of a cluster take parts of the keys and join over
 // distributed shared memory.
-//   warps 0-3    loaders: rows of 128-key blocks by cp.async (any page size and stride), three
-//                blocks ahead, expanded into 128B-swizzled f16 tiles
+//   warps 0-3    loaders, by cp.async (any page size and stride).  e4m3: 128-key blocks, three ahead,
+//                expanded into 128B-swizzled f16 tiles; bf16: 96-key blocks, four ahead, whose rows go
+//                straight into their tiles (three of the warps)
 //   warps 4-11   softmax, one warpgroup per 128-row tile: thread t owns query row t
-//   warp 12      tcgen05 issuer: S = Q K^T (M 128, N 128, K 64) of the next block is issued before
-//                O += P V (M 128, N 64, K 128, P from TMEM) of this one
-//   warps 14-15  bf16 pages: loaders of K, whose rows go straight into their tile
-// Measured with 64 query heads on 8 KV heads: 4096 rows over 12288 cached keys 1.59 ms with e4m3 pages
-// (606 TFLOP/s), 1.68 ms with bf16 (2.15 ms before K had loaders of its own).  The exponentials alone
-// take 0.86 ms (16 a cycle and SM), the softmax and the products without loaders 1.30 ms, loaders and
-// products without softmax 0.85 ms (e4m3).  The rest is the two getting in each other's way: issue
-// slots of the softmax's dependent instructions, and the instruction cache (3 to 7 % misses).  Tried
-// and slower: K loaders of their own for e4m3 too (1.74 ms, 14 % misses), four softmax streams of 64
-// keys (1.83 ms), rolled loops in the issuer (1.86 ms), spinning or sleeping waits.
-// TMEM columns: S[A] 0, S[B] 128, P[A] 256, P[B] 320 (f16 pairs), O[A] 384, O[B] 448.
+//   warp 12      tcgen05 issuer: S = Q K^T (M 128, N a block, K 64) of the next block is issued before
+//                O += P V (M 128, N 64, K a block, P from TMEM) of this one
+// Measured with 64 query heads on 8 KV heads: 4096 rows over 12288 cached keys 1.60 ms with e4m3 pages
+// (602 TFLOP/s), 1.75 ms with bf16.  The exponentials alone take 0.86 ms (16 a cycle and SM), the
+// softmax and the products without loaders 1.30 ms, loaders and products without softmax 0.85 ms
+// (e4m3).  The rest is the two getting in each other's way: issue slots of the softmax's dependent
+// instructions, and the instruction cache (3 to 7 % misses).  Tried and slower: K loaders of their own
+// for e4m3 (1.74 ms, 14 % misses), four softmax streams of 64 keys (1.83 ms), rolled loops in the
+// issuer (1.86 ms), spinning or sleeping waits.
 //
-// P and V enter the second product as f16: bf16's 8 bits for P would cost as much precision as the
-// rounding of the output.  V is scaled by a power of two that follows the largest magnitude the
-// CTA has loaded (its unit 2^u; O is rescaled when u grows), so that f16 holds all of it:
-//   e4m3 pages: V' = code * 2^(e - u), K' = code * 2^(e - ek) with ek the block's largest exponent;
-//               both exact while a key's exponent is within kWideRange of the largest
-//   bf16 pages: V' = v * 2^-u with the largest |V'| in [2^8, 2^9); K and Q stay bf16
-// The softmax reference is the running maximum itself: the largest p is 2^10 exactly, so that a row
-// that one key dominates comes out as that key's value, and f16 keeps 11 bits down to 2^-24 of it.
+// One bf16 P would cost as much precision as the rounding of the output.
+//   bf16 pages: K, V and Q as they are; P as two bf16 numbers, its first 8 bits and the next 8 (two
+//               products), so that values of every magnitude keep their bits, next to any others.  P
+//               takes as many TMEM columns as S and lies over it; two S of 96 columns a tile let the
+//               next block's product start before this one's P is used (one S of 128: 2.04 ms).
+//               TMEM: S / P of tile A 0 and 96, of tile B 192 and 288, O 384 and 448.
+//   e4m3 pages: P as f16.  V' = code * 2^(e - u), with u the largest exponent the CTA has loaded (O is
+//               rescaled when u grows), K' = code * 2^(e - ek) with ek the block's largest exponent;
+//               both exact while a key's exponent is within kWideRange of the largest.
+//               TMEM: S 0 and 128, P 256 and 320, O 384 and 448.
+// The softmax reference is the running maximum itself: the largest p is 1 (bf16) or 2^10 (f16, which so
+// keeps 11 bits down to 2^-24 of it), and a row that one key dominates comes out as that key's value.
 //
 // Rows that do not see a value must not meet it as 0 * inf: blocks that are not fully visible to
 // the whole span have such values cleared by the loaders and their keys reported; rows that do see
-// one, and spans of too wide a range, are taken key by key at the end.
+// one, and e4m3 spans of too wide a range, are taken key by key at the end.
 #include <cooperative_groups.h>
 
 #include "common.h"
@@ -45,35 +48,45 @@ namespace af3 {
 namespace paged {
 
 constexpr int kChunkThreads = 512;
-constexpr int kBK = 128;         // keys of a block
-constexpr int kST = 4;           // f16 K/V stages
-constexpr int kRaw = 3;          // raw blocks in flight
-constexpr int kTile = kBK * kD * 2;  // 16 KB: a 16-bit K, V or Q tile; also a raw block
-constexpr uint32_t kColS = 0, kColP = 256, kColO = 384;
-constexpr float kTopLog2 = 10.f;  // the largest p of a row is 2^10
+constexpr int kQTile = 128 * kD * 2;  // 16 KB: 128 rows of Q
+constexpr uint32_t kColO = 384;
+constexpr float kTopLog2 = 10.f;  // the largest p of a row is 2^10 (e4m3 pages; 1 for bf16)
 
-struct ChunkSmem {
+// Blocks, stages and where things lie.
+template <bool FP8>
+struct Cfg {
+  static constexpr int kBK = FP8 ? 128 : 96;     // keys of a block
+  static constexpr int kST = FP8 ? 4 : 6;        // stages of K/V tiles
+  static constexpr int kAhead = FP8 ? 3 : 4;     // blocks whose copies are in flight
+  static constexpr int kLoaders = kBK / 32;      // warps, 32 keys each
+  static constexpr int kTile = kBK * kD * 2;     // a 16-bit tile of K or V; e4m3: also a raw block
+  // shared memory
   static constexpr int Q = 0;                    // 2 tiles
-  static constexpr int K = Q + 2 * kTile;        // kST tiles
+  static constexpr int K = Q + 2 * kQTile;       // kST tiles
   static constexpr int V = K + kST * kTile;      // kST tiles
-  static constexpr int RAW = V + kST * kTile;    // kRaw raw blocks: own 16-byte pieces of each loader thread
-  static constexpr int INFO = RAW + kRaw * kTile;
+  static constexpr int RAW = V + kST * kTile;    // e4m3: kAhead raw blocks, own 16-byte pieces of each loader thread
+  static constexpr int kBytes = RAW + (FP8 ? kAhead * kTile : 0);
+  static_assert(256 * kD * 4 <= kST * kTile, "a CTA's parts lie over its K tiles");
+  // TMEM columns of block c's S and P of tile x
+  __device__ static uint32_t col_s(int x, int c) { return FP8 ? x * 128 : x * 192 + (c & 1) * 96; }
+  __device__ static uint32_t col_p(int x, int c) { return FP8 ? 256 + x * 64 : col_s(x, c); }
 };
 
 struct StageInfo {
   uint32_t there[4];   // keys that exist and lie in the span's range, but for the broken ones
   uint32_t broken[4];  // those whose V is not finite (cleared), in blocks not seen by every row
-  float kmul;          // 2^ek (e4m3)
-  int unit;            // V' is in units of 2^unit
+  float kmul;          // e4m3: 2^ek
+  int unit;            // e4m3: V' is in units of 2^unit
 };
 
+constexpr int kMaxST = 6;
 struct ChunkBars {
-  uint64_t q_full, kv_full[kST], kv_empty[kST], s_full[2], s_free[2], p_full[2], o_ready[2];
+  uint64_t q_full, kv_full[kMaxST], kv_empty[kMaxST], s_full[2], s_free[2], p_full[2], o_ready[2];
   uint32_t tmem;
   int abort_flag;
   int wide;
   uint32_t red[2][4];
-  StageInfo info[kST];
+  StageInfo info[kMaxST];
   float row_m[256], row_l[256];
 };
 static_assert(sizeof(ChunkBars) <= 4096, "");
@@ -130,6 +143,7 @@ struct Tile {
   int jlo, jhi;  // blocks, absolute; empty when jhi <= jlo
 };
 
+template <int kBK>
 __device__ __forceinline__ Tile make_tile(const Args& a, const Seq& s, int tok0, int tokens, int kv_lo, int b0, int b1) {
   Tile t;
   t.tok0 = tok0;
@@ -170,31 +184,41 @@ template <bool FP8, int X>
 __device__ __forceinline__ bool issue_s(Issue& t, int j, int st, uint32_t tmem, uint32_t sq, uint32_t sk0, ChunkBars* b,
                                         int* err) {
   if (j < t.jlo || j >= t.jhi) return true;
-  if (t.n_s > 0 && !mbar_wait(&b->s_free[X], (t.n_s - 1) & 1, err, &b->abort_flag)) return false;
+  using C = Cfg<FP8>;
+  // e4m3: once S has been read; bf16: once the block before the last, whose P lies there, is done
+  if constexpr (FP8) {
+    if (t.n_s > 0 && !mbar_wait(&b->s_free[X], (t.n_s - 1) & 1, err, &b->abort_flag)) return false;
+  } else {
+    if (t.n_s > 1 && !mbar_wait(&b->o_ready[X], t.n_s & 1, err, &b->abort_flag)) return false;
+  }
   tc_fence_after();
-  constexpr uint32_t idesc = FP8 ? make_idesc_f16(128, kBK, false, false) : make_idesc_bf16(128, kBK, false, false);
-  const uint32_t q = sq + X * kTile, k = sk0 + st * kTile;
+  constexpr uint32_t idesc = FP8 ? make_idesc_f16(128, C::kBK, false, false) : make_idesc_bf16(128, C::kBK, false, false);
+  const uint32_t q = sq + X * kQTile, k = sk0 + st * C::kTile, s = tmem + C::col_s(X, t.n_s);
 #pragma unroll
   for (int kk = 0; kk < kD / 16; ++kk)
-    umma_f16(tmem + kColS + X * kBK, make_smem_desc(q + kk * 32, 16, 1024, kLayoutSW128),
+    umma_f16(s, make_smem_desc(q + kk * 32, 16, 1024, kLayoutSW128),
              make_smem_desc(k + kk * 32, 16, 1024, kLayoutSW128), idesc, kk > 0);
   umma_commit(&b->s_full[X]);
   ++t.n_s;
   return true;
 }
 
-template <int X>
+template <bool FP8, int X>
 __device__ __forceinline__ bool issue_pv(Issue& t, int j, int st, uint32_t tmem, uint32_t sv0, ChunkBars* b, int* err) {
   if (j < t.jlo || j >= t.jhi) return true;
+  using C = Cfg<FP8>;
   if (!mbar_wait(&b->p_full[X], t.n_pv & 1, err, &b->abort_flag)) return false;
   tc_fence_after();
-  constexpr uint32_t idesc = make_idesc_f16(128, kD, false, true);
-  const uint32_t v = sv0 + st * kTile;
+  constexpr uint32_t idesc = FP8 ? make_idesc_f16(128, kD, false, true) : make_idesc_bf16(128, kD, false, true);
+  const uint32_t v = sv0 + st * C::kTile, p = tmem + C::col_p(X, t.n_pv);
   const uint32_t first = t.n_pv > 0 ? 1u : 0u;
 #pragma unroll
-  for (int kk = 0; kk < kBK / 16; ++kk)
-    umma_f16_tmem_a(tmem + kColO + X * kD, tmem + kColP + X * 64 + kk * 8,
-                    make_smem_desc(v + kk * 2048, 8192, 1024, kLayoutSW128), idesc, kk > 0 ? 1u : first);
+  for (int term = 0; term < (FP8 ? 1 : 2); ++term) {
+#pragma unroll
+    for (int kk = 0; kk < C::kBK / 16; ++kk)
+      umma_f16_tmem_a(tmem + kColO + X * kD, p + term * (C::kBK / 2) + kk * 8,
+                      make_smem_desc(v + kk * 2048, 8192, 1024, kLayoutSW128), idesc, term + kk > 0 ? 1u : first);
+  }
   umma_commit(&b->o_ready[X]);
   ++t.n_pv;
   return true;
@@ -215,12 +239,11 @@ __device__ __forceinline__ int page_of(const Args& a, const int* table, int j, i
   return page;
 }
 
-// Starts the copies of keys key0 .. key0 + 31 of `pool`: piece i of lane l, rows 8 i + l / 4 (e4m3,
-// 16 codes each) or 4 i + l / 8 (bf16, 8 values), goes to own + i * pitch (and `pool2`'s pieces after
-// `pool`'s, e4m3), or with TILE into rows r0 .. r0 + 31 of a swizzled tile.
-template <bool FP8, bool TILE>
-__device__ __forceinline__ Rows load_rows(const Args& a, const uint8_t* pool, const uint8_t* pool2, int page, int g, int key0,
-                                          uint32_t dst, int pitch_or_r0) {
+// Starts the copies of keys key0 .. key0 + 31.  e4m3: 16 codes a piece, piece i of lane l is of row
+// 8 i + l / 4; V's go to own + i * 2048 (dst), K's after them.  bf16: 8 values a piece, of row
+// 4 i + l / 8, into rows r0 .. r0 + 31 of the swizzled tiles of K (dst) and V (as far behind).
+template <bool FP8>
+__device__ __forceinline__ Rows load_rows(const Args& a, int page, int g, int key0, uint32_t dst, int r0) {
   const int lane = threadIdx.x & 31;
   const bool on = (uint32_t)page < (uint32_t)a.p.num_pages;
   int64_t row = 0, sc = 0;
@@ -233,18 +256,20 @@ __device__ __forceinline__ Rows load_rows(const Args& a, const uint8_t* pool, co
   Rows h;
   h.there = __ballot_sync(0xffffffffu, on);
   h.scale = sc;
-  constexpr int kPer = FP8 ? 4 : 8;  // pieces of a row = rows a piece index steps over, inverted
+  constexpr int kPer = FP8 ? 4 : 8;  // pieces of a row
   const int c = lane % kPer;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int r = (32 / kPer) * i + lane / kPer;
     const int64_t off = __shfl_sync(0xffffffffu, row, r) + c * 16;
     const bool there = (h.there >> r) & 1u;
-    if constexpr (TILE) {
-      cp16(dst + sw128(pitch_or_r0 + r, c), pool + off, there);
+    if constexpr (FP8) {
+      cp16(dst + i * 2048, a.p.v + off, there);
+      cp16(dst + (4 + i) * 2048, a.p.k + off, there);
     } else {
-      cp16(dst + i * pitch_or_r0, pool + off, there);
-      if constexpr (FP8) cp16(dst + (4 + i) * pitch_or_r0, pool2 + off, there);
+      const uint32_t at = dst + sw128(r0 + r, c);
+      cp16(at, a.p.k + off, there);
+      cp16(at + (Cfg<false>::V - Cfg<false>::K), a.p.v + off, there);
     }
   }
   return h;
@@ -258,6 +283,30 @@ __device__ __forceinline__ uint32_t any_of_groups(uint32_t x, int n) {
 
 __device__ __forceinline__ void st4(uint32_t addr, uint32_t x, uint32_t y, uint32_t z, uint32_t u) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(u));
+}
+
+// Zeroes what is not finite in rows r0 .. r0 + 31 of a bf16 tile of V, each lane in the pieces that
+// it has copied; the keys (bits) that had something.
+__device__ __forceinline__ uint32_t clear_tile_rows(uint32_t tile, int r0) {
+  const int lane = threadIdx.x & 31;
+  uint32_t broken = 0;
+#pragma unroll 1
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t at = tile + sw128(r0 + 4 * i + (lane >> 3), lane & 7);
+    const uint4 w = lds4(at);
+    uint32_t x[4] = {w.x, w.y, w.z, w.w}, bad = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t m = __vcmpeq2(x[e] & 0x7f807f80u, 0x7f807f80u);
+      bad |= m;
+      x[e] &= ~m;
+    }
+    if (bad) st4(at, x[0], x[1], x[2], x[3]);
+    const uint32_t q = any_of_groups(__ballot_sync(0xffffffffu, bad != 0), 8);  // bit 8 r: key 4 i + r
+#pragma unroll
+    for (int r = 0; r < 4; ++r) broken |= ((q >> (8 * r)) & 1u) << (4 * i + r);
+  }
+  return broken;
 }
 
 // 16 e4m3 codes -> 16 f16 scaled by mul, into chunks 2c and 2c + 1 of row r.
@@ -278,6 +327,8 @@ __device__ __forceinline__ void expand16(uint32_t tile, int r, int c, const uint
 template <bool FP8>
 __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Args a, const int tokens, const int splits,
                                                                       int* err) {
+  using C = Cfg<FP8>;
+  constexpr int kBK = C::kBK, kST = C::kST, kAhead = C::kAhead, kTile = C::kTile;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ ChunkBars bars;
@@ -303,12 +354,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
   const int per = (nb + splits - 1) / splits;
   const int b0 = min(rank * per, nb), b1 = min(b0 + per, nb);
   const int* table = a.table + (int64_t)sb * a.ld_table;
-  const Tile tl[2] = {make_tile(a, sq, tok0, tokens, lo, b0, b1), make_tile(a, sq, tok0 + tokens, tokens, lo, b0, b1)};
+  const Tile tl[2] = {make_tile<kBK>(a, sq, tok0, tokens, lo, b0, b1), make_tile<kBK>(a, sq, tok0 + tokens, tokens, lo, b0, b1)};
 
   if (warp == 0 && lane == 0) {
     mbar_init(&b->q_full, 8);
     for (int s = 0; s < kST; ++s) {
-      mbar_init(&b->kv_full[s], FP8 ? 4 : 6);
+      mbar_init(&b->kv_full[s], C::kLoaders);
       mbar_init(&b->kv_empty[s], 1);
     }
     for (int x = 0; x < 2; ++x) {
@@ -334,30 +385,69 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
   // a block is seen in full by every row of the span when it lies in [full_lo, full_hi)
   const int full_lo = a.window > 0 ? pos0 + ntok - a.window : 0, full_hi = min(pos0 + 1, sq.key_end);
 
-  // registers (launch: 512 x 128): loaders 72, softmax 2 x 184, issuer and K loaders 72
-  if (warp < 4) {
+  // registers (launch: 512 x 128): loaders 72, softmax 2 x 184, issuer 72
+  if (!FP8 && warp < 4) {
+    setmaxnreg_dec<72>();
+    if (warp < C::kLoaders) {
+      const int w = warp, key0 = lo + 32 * w;
+      bool dead = false;
+      uint32_t there[kAhead];
+      int next_page = b0 < b1 ? page_of(a, table, key0 + lane + b0 * kBK, hi) : -1;
+      auto load = [&](int j) -> uint32_t {
+        const int page = next_page;
+        if (j + 1 < b1) next_page = page_of(a, table, key0 + lane + (j + 1) * kBK, hi);
+        return load_rows<false>(a, page, g, key0 + j * kBK, sbase + C::K + ((j - b0) % kST) * kTile, 32 * w).there;
+      };
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        there[i] = b0 + i < b1 ? load(b0 + i) : 0u;
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      }
+#pragma unroll 1
+      for (int j = b0; j < b1; ++j) {
+        const int n = j - b0, st = n % kST, m = n + kAhead, k0 = lo + j * kBK;
+        asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
+        uint32_t broken = 0;  // keys of this warp
+        if (k0 < full_lo || k0 + kBK > full_hi) broken = clear_tile_rows(sbase + C::V + st * kTile, 32 * w);
+        if (lane == 0) {
+          b->info[st].there[w] = there[0] & ~broken;
+          b->info[st].broken[w] = broken;
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&b->kv_full[st]);
+#pragma unroll
+        for (int i = 0; i < kAhead - 1; ++i) there[i] = there[i + 1];
+        there[kAhead - 1] = 0;
+        if (j + kAhead < b1) {
+          if (!dead && m >= kST && !mbar_wait(&b->kv_empty[m % kST], ((m / kST) & 1) ^ 1, err, &b->abort_flag)) dead = true;
+          there[kAhead - 1] = load(j + kAhead);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      }
+    }
+  } else if (warp < 4) {
     setmaxnreg_dec<72>();
     const int w = warp;
-    constexpr int kPieces = FP8 ? 4 : 8;
-    uint32_t top = 0;  // largest e8m0 byte (e4m3) or biased exponent (bf16) so far
+    uint32_t top = 0;  // largest scale byte of V so far
     bool dead = false;
-    Rows ah[kRaw];
+    Rows ah[kAhead];
     // Scale bytes of the block to expand.  Those of the next block are asked for at the top of a round
     // and moved here at its end: a move right after the load would wait for it (1000 cycles a block).
     uint32_t byte = 0, kbyte = 0;
     auto fetch_scale = [&](const uint8_t* from, const Rows& h) -> uint32_t {
-      return FP8 ? load_byte(from + h.scale, (h.there >> lane) & 1u) : 0u;
+      return load_byte(from + h.scale, (h.there >> lane) & 1u);
     };
     const int key0 = lo + 32 * w;
-    int pages[kRaw];
+    int pages[kAhead];
 #pragma unroll
-    for (int i = 0; i < kRaw; ++i) pages[i] = b0 + i < b1 ? page_of(a, table, key0 + lane + (b0 + i) * kBK, hi) : -1;
-    int next_page = b0 + kRaw < b1 ? page_of(a, table, key0 + lane + (b0 + kRaw) * kBK, hi) : -1;
-    const uint32_t own0 = sbase + ChunkSmem::RAW + (32 * w + lane) * 16;
+    for (int i = 0; i < kAhead; ++i) pages[i] = b0 + i < b1 ? page_of(a, table, key0 + lane + (b0 + i) * kBK, hi) : -1;
+    int next_page = b0 + kAhead < b1 ? page_of(a, table, key0 + lane + (b0 + kAhead) * kBK, hi) : -1;
+    const uint32_t own0 = sbase + C::RAW + (32 * w + lane) * 16;
 #pragma unroll
-    for (int i = 0; i < kRaw; ++i) {
+    for (int i = 0; i < kAhead; ++i) {
       ah[i] = Rows{0, 0};
-      if (b0 + i < b1) ah[i] = load_rows<FP8, false>(a, a.p.v, a.p.k, pages[i], g, key0 + (b0 + i) * kBK, own0 + i * kTile, 2048);
+      if (b0 + i < b1) ah[i] = load_rows<true>(a, pages[i], g, key0 + (b0 + i) * kBK, own0 + i * kTile, 0);
       asm volatile("cp.async.commit_group;" ::: "memory");
     }
     byte = fetch_scale(a.p.vs, ah[0]);
@@ -366,88 +456,34 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
     for (int j = b0; j < b1; ++j) {
       const int n = j - b0, st = n % kST;
       const uint32_t next_byte = fetch_scale(a.p.vs, ah[1]), next_kbyte = fetch_scale(a.p.ks, ah[1]);
-      const uint32_t own = own0 + raw_slot * kTile, vtile = sbase + ChunkSmem::V + st * kTile;
-      asm volatile("cp.async.wait_group %0;" ::"n"(kRaw - 1) : "memory");
+      const uint32_t own = own0 + raw_slot * kTile, vtile = sbase + C::V + st * kTile;
+      asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
       const int k0 = lo + j * kBK;
       const bool partial = k0 < full_lo || k0 + kBK > full_hi;
       uint32_t broken = 0;  // keys of this warp
-      uint4 v[kPieces];
+      uint4 v[4];
 #pragma unroll
-      for (int i = 0; i < kPieces; ++i) v[i] = lds4(own + i * 2048);
-      // ---- largest exponent of the block, and the smallest that is not of zeros: of a row (e4m3),
-      // of 8 values of a row (bf16)
-      uint32_t vmax = 0, vmin = 255;
-      if constexpr (FP8) {
-        if (partial) {
+      for (int i = 0; i < 4; ++i) v[i] = lds4(own + i * 2048);
+      if (partial) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t* x = reinterpret_cast<uint32_t*>(&v[i]);
-            bool bad = false;
+        for (int i = 0; i < 4; ++i) {
+          uint32_t* x = reinterpret_cast<uint32_t*>(&v[i]);
+          bool bad = false;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const uint32_t m = __vcmpeq4(x[e] & 0x7f7f7f7fu, 0x7f7f7f7fu);
-              bad |= m != 0;
-              x[e] &= ~m;
-            }
-            const uint32_t q = any_of_groups(__ballot_sync(0xffffffffu, bad), 4);  // bit 4 r: key 8 i + r
-#pragma unroll
-            for (int r = 0; r < 8; ++r) broken |= ((q >> (4 * r)) & 1u) << (8 * i + r);
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t m = __vcmpeq4(x[e] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+            bad |= m != 0;
+            x[e] &= ~m;
           }
+          const uint32_t q = any_of_groups(__ballot_sync(0xffffffffu, bad), 4);  // bit 4 r: key 8 i + r
+#pragma unroll
+          for (int r = 0; r < 8; ++r) broken |= ((q >> (4 * r)) & 1u) << (8 * i + r);
         }
-        const uint32_t vb = ((broken >> lane) & 1u) || byte == 255u ? 0u : byte;
-        vmax = vb;
-        vmin = vb ? vb : 255u;
-      } else {
-        uint32_t all = 0, least = 0xffffu;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const uint32_t m2 = __vmaxu2(__vmaxu2(v[i].x & 0x7fff7fffu, v[i].y & 0x7fff7fffu),
-                                       __vmaxu2(v[i].z & 0x7fff7fffu, v[i].w & 0x7fff7fffu));
-          const uint32_t m = max(m2 & 0xffffu, m2 >> 16);
-          all = max(all, m);
-          least = min(least, m - 1u);  // 0 wraps to the largest
-        }
-        if (__any_sync(0xffffffffu, all >= 0x7f80u)) {  // something is not finite
-          all = 0;
-          least = 0xffffu;
-#pragma unroll 1
-          for (int i = 0; i < 8; ++i) {
-            const uint4 raw = lds4(own + i * 2048);
-            const uint32_t x[4] = {raw.x, raw.y, raw.z, raw.w};
-            uint32_t m = 0;
-            bool bad = false;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const uint32_t f = __vcmpeq2(x[e] & 0x7f807f80u, 0x7f807f80u);
-              const uint32_t fin = x[e] & ~f & 0x7fff7fffu;
-              m = max(m, max(fin & 0xffffu, fin >> 16));
-              bad |= f != 0;
-            }
-            if (bad && partial) {
-              const uint32_t y[4] = {x[0] & ~__vcmpeq2(x[0] & 0x7f807f80u, 0x7f807f80u), x[1] & ~__vcmpeq2(x[1] & 0x7f807f80u, 0x7f807f80u),
-                                     x[2] & ~__vcmpeq2(x[2] & 0x7f807f80u, 0x7f807f80u), x[3] & ~__vcmpeq2(x[3] & 0x7f807f80u, 0x7f807f80u)};
-              st4(own + i * 2048, y[0], y[1], y[2], y[3]);
-            }
-            const uint32_t q = any_of_groups(__ballot_sync(0xffffffffu, bad && partial), 8);  // bit 8 r: key 4 i + r
-#pragma unroll
-            for (int r = 0; r < 4; ++r) broken |= ((q >> (8 * r)) & 1u) << (4 * i + r);
-            all = max(all, m);
-            least = min(least, m - 1u);
-          }
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = lds4(own + i * 2048);
-        }
-        vmax = all >> 7;
-        vmin = least >= 0xffffu ? 255u : (least + 1u) >> 7;
       }
-      vmax = __reduce_max_sync(0xffffffffu, vmax);
-      vmin = __reduce_min_sync(0xffffffffu, vmin);
-      uint32_t kmax = 0, kmin = 255;
-      if constexpr (FP8) {
-        const uint32_t kb = kbyte == 255u ? 0u : kbyte;
-        kmax = __reduce_max_sync(0xffffffffu, kb);
-        kmin = __reduce_min_sync(0xffffffffu, kb ? kb : 255u);
-      }
+      // ---- largest exponent of the block, and the smallest that is not of zeros
+      const uint32_t vb = ((broken >> lane) & 1u) || byte == 255u ? 0u : byte, kb = kbyte == 255u ? 0u : kbyte;
+      const uint32_t vmax = __reduce_max_sync(0xffffffffu, vb), vmin = __reduce_min_sync(0xffffffffu, vb ? vb : 255u);
+      uint32_t kmax = __reduce_max_sync(0xffffffffu, kb), kmin = __reduce_min_sync(0xffffffffu, kb ? kb : 255u);
       if (lane == 0) b->red[n & 1][w] = vmax | (vmin << 8) | (kmax << 16) | (kmin << 24);
       named_barrier_sync(1, 128);
       uint32_t most = 0, least = 255;
@@ -461,110 +497,53 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
       }
       top = max(top, most);
       if (threadIdx.x == 0) {
-        if (least != 255u && (int)(top - least) > (FP8 ? kWideRange : kWideRangeBf16)) b->wide = 1;
-        if (FP8 && kmin != 255u && (int)(kmax - kmin) > kWideRange) b->wide = 1;
+        if (least != 255u && (int)(top - least) > kWideRange) b->wide = 1;
+        if (kmin != 255u && (int)(kmax - kmin) > kWideRange) b->wide = 1;
       }
       if (!dead && n >= kST && !mbar_wait(&b->kv_empty[st], ((n / kST) & 1) ^ 1, err, &b->abort_flag)) dead = true;
       // ---- expand into the f16 tile
-      if constexpr (FP8) {
-        // (each key's lane works out its factor, and all of them travel before the first store: left
-        // to the loop below, the stores kept the rows one after the other)
-        const uint32_t mine = h2_pow2(min((int)byte - (int)top, 0));
-        uint32_t mul[4];
+      // (each key's lane works out its factor, and all of them travel before the first store: left
+      // to the loop below, the stores kept the rows one after the other)
+      const uint32_t mine = h2_pow2(min((int)byte - (int)top, 0)), kmine = h2_pow2(min((int)kbyte - (int)kmax, 0));
+      uint32_t mul[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) mul[i] = __shfl_sync(0xffffffffu, mine, 8 * i + (lane >> 2));
+      for (int i = 0; i < 4; ++i) mul[i] = __shfl_sync(0xffffffffu, mine, 8 * i + (lane >> 2));
 #pragma unroll
-        for (int i = 0; i < 4; ++i) expand16(vtile, 32 * w + 8 * i + (lane >> 2), lane & 3, v[i], mul[i]);
+      for (int i = 0; i < 4; ++i) expand16(vtile, 32 * w + 8 * i + (lane >> 2), lane & 3, v[i], mul[i]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = lds4(own + (4 + i) * 2048);
-        const uint32_t kmine = h2_pow2(min((int)kbyte - (int)kmax, 0));
+      for (int i = 0; i < 4; ++i) v[i] = lds4(own + (4 + i) * 2048);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) mul[i] = __shfl_sync(0xffffffffu, kmine, 8 * i + (lane >> 2));
+      for (int i = 0; i < 4; ++i) mul[i] = __shfl_sync(0xffffffffu, kmine, 8 * i + (lane >> 2));
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          expand16(sbase + ChunkSmem::K + st * kTile, 32 * w + 8 * i + (lane >> 2), lane & 3, v[i], mul[i]);
-      } else {
-        // largest |V'| in [2^8, 2^9): v * 2^(135 - top)
-        const float f = pow2i(135 - (int)max(top, 9u));
-        const uint64_t ff = pk2(f, f);
-        const int c = lane & 7;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const uint32_t x[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-          uint32_t o[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float p0, p1;
-            upk2(fma2(pk2(__uint_as_float(x[e] << 16), __uint_as_float(x[e] & 0xffff0000u)), ff, pk2(0.f, 0.f)), p0, p1);
-            o[e] = h2_of(p0, p1);
-          }
-          st4(vtile + sw128(32 * w + 4 * i + (lane >> 3), c), o[0], o[1], o[2], o[3]);
-        }
-      }
+      for (int i = 0; i < 4; ++i)
+        expand16(sbase + C::K + st * kTile, 32 * w + 8 * i + (lane >> 2), lane & 3, v[i], mul[i]);
       if (lane == 0) {
         b->info[st].there[w] = ah[0].there & ~broken;
         b->info[st].broken[w] = broken;
       }
-      if (threadIdx.x == 0) b->info[st].kmul = FP8 ? pow2i((int)kmax - 127) : 1.f;
-      if (threadIdx.x == 0) b->info[st].unit = FP8 ? (int)top - 127 : (int)max(top, 9u) - 135;
+      if (threadIdx.x == 0) b->info[st].kmul = pow2i((int)kmax - 127);
+      if (threadIdx.x == 0) b->info[st].unit = (int)top - 127;
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&b->kv_full[st]);
       // ---- refill
 #pragma unroll
-      for (int i = 0; i < kRaw - 1; ++i) ah[i] = ah[i + 1];
-      ah[kRaw - 1] = Rows{0, 0};
-      if (j + kRaw < b1) {
+      for (int i = 0; i < kAhead - 1; ++i) ah[i] = ah[i + 1];
+      ah[kAhead - 1] = Rows{0, 0};
+      if (j + kAhead < b1) {
         const int page = next_page;
-        if (j + kRaw + 1 < b1) next_page = page_of(a, table, key0 + lane + (j + kRaw + 1) * kBK, hi);
-        ah[kRaw - 1] = load_rows<FP8, false>(a, a.p.v, a.p.k, page, g, key0 + (j + kRaw) * kBK, own, 2048);
+        if (j + kAhead + 1 < b1) next_page = page_of(a, table, key0 + lane + (j + kAhead + 1) * kBK, hi);
+        ah[kAhead - 1] = load_rows<true>(a, page, g, key0 + (j + kAhead) * kBK, own, 0);
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
       byte = next_byte;
       kbyte = next_kbyte;
-      raw_slot = raw_slot + 1 == kRaw ? 0 : raw_slot + 1;
+      raw_slot = raw_slot + 1 == kAhead ? 0 : raw_slot + 1;
     }
   } else if (warp >= 12) {
     setmaxnreg_dec<72>();
-    if (!FP8 && warp >= 14) {  // bf16 K: 64 keys a warp, in two groups of 32, straight into their tile
-      const int w = warp - 14;
-      bool dead = false;
-      const int key0 = lo + 64 * w + lane;
-      int next_page[2];
-#pragma unroll
-      for (int u = 0; u < 2; ++u) next_page[u] = b0 < b1 ? page_of(a, table, key0 + 32 * u + b0 * kBK, hi) : -1;
-      auto load = [&](int j) {
-        const int page[2] = {next_page[0], next_page[1]};
-        if (j + 1 < b1) {
-#pragma unroll
-          for (int u = 0; u < 2; ++u) next_page[u] = page_of(a, table, key0 + 32 * u + (j + 1) * kBK, hi);
-        }
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-          load_rows<FP8, true>(a, a.p.k, nullptr, page[u], g, lo + 64 * w + 32 * u + j * kBK,
-                               sbase + ChunkSmem::K + ((j - b0) % kST) * kTile, 64 * w + 32 * u);
-      };
-#pragma unroll 1
-      for (int i = 0; i < kRaw; ++i) {
-        if (b0 + i < b1) load(b0 + i);
-        asm volatile("cp.async.commit_group;" ::: "memory");
-      }
-#pragma unroll 1
-      for (int j = b0; j < b1; ++j) {
-        const int n = j - b0, m = n + kRaw;
-        asm volatile("cp.async.wait_group %0;" ::"n"(kRaw - 1) : "memory");
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&b->kv_full[n % kST]);
-        if (j + kRaw < b1) {
-          if (!dead && m >= kST && !mbar_wait(&b->kv_empty[m % kST], ((m / kST) & 1) ^ 1, err, &b->abort_flag)) dead = true;
-          load(j + kRaw);
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-      }
-    }
     if (warp == 12 && b1 > b0 && elect_one_sync()) {
-      const uint32_t sqa = sbase + ChunkSmem::Q, sk0 = sbase + ChunkSmem::K, sv0 = sbase + ChunkSmem::V;
+      const uint32_t sqa = sbase + C::Q, sk0 = sbase + C::K, sv0 = sbase + C::V;
       Issue ta{tl[0].jlo, tl[0].jhi, 0, 0}, tb{tl[1].jlo, tl[1].jhi, 0, 0};
       bool ok = mbar_wait(&b->q_full, 0, err, &b->abort_flag) && mbar_wait(&b->kv_full[0], 0, err, &b->abort_flag);
       ok = ok && issue_s<FP8, 0>(ta, b0, 0, tmem, sqa, sk0, b, err) && issue_s<FP8, 1>(tb, b0, 0, tmem, sqa, sk0, b, err);
@@ -573,9 +552,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
         const bool next = j + 1 < b1;
         if (next) ok = mbar_wait(&b->kv_full[sn], ((n + 1) / kST) & 1, err, &b->abort_flag);
         if (ok && next) ok = issue_s<FP8, 0>(ta, j + 1, sn, tmem, sqa, sk0, b, err);
-        ok = ok && issue_pv<0>(ta, j, st, tmem, sv0, b, err);
+        ok = ok && issue_pv<FP8, 0>(ta, j, st, tmem, sv0, b, err);
         if (ok && next) ok = issue_s<FP8, 1>(tb, j + 1, sn, tmem, sqa, sk0, b, err);
-        ok = ok && issue_pv<1>(tb, j, st, tmem, sv0, b, err);
+        ok = ok && issue_pv<FP8, 1>(tb, j, st, tmem, sv0, b, err);
         umma_commit(&b->kv_empty[st]);
       }
     }
@@ -594,7 +573,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
     float qmul = a.scale_log2;
     {  // this row of Q into its tile
       const uint4* src = reinterpret_cast<const uint4*>(a.q + (int64_t)tok * a.ld_q + (int64_t)h * kD);
-      const uint32_t dst = sbase + ChunkSmem::Q + x * kTile;
+      const uint32_t dst = sbase + C::Q + x * kQTile;
       uint4 w[8];
 #pragma unroll
       for (int c = 0; c < 8; ++c) w[c] = real ? src[c] : make_uint4(0, 0, 0, 0);
@@ -622,8 +601,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
       if (lane == 0) mbar_arrive(&b->q_full);
     }
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_addr = tmem + lane_base + kColS + x * kBK;
-    const uint32_t p_addr = tmem + lane_base + kColP + x * 64;
     const uint32_t o_addr = tmem + lane_base + kColO + x * kD;
     // blocks [k0, k0 + 128) with every key visible to every row of the tile
     const int tile_lo = a.window > 0 ? max(t.pos0 + t.ntok - a.window, 0) - lo : -lo;
@@ -638,32 +615,28 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
           !mbar_wait(&b->kv_full[st], ((j - b0) / kST) & 1, err, &b->abort_flag)) { ok = false; break; }
       tc_fence_after();
       const StageInfo* info = &b->info[st];
+      const uint32_t s_addr = tmem + lane_base + C::col_s(x, c), p_addr = tmem + lane_base + C::col_p(x, c);
       float sv[kBK];
       {
-        uint32_t r0[32], r1[32], r2[32], r3[32];
-        tmem_ld_32x32b_x32(s_addr, r0);
-        tmem_ld_32x32b_x32(s_addr + 32, r1);
-        tmem_ld_32x32b_x32(s_addr + 64, r2);
-        tmem_ld_32x32b_x32(s_addr + 96, r3);
+        uint32_t r[kBK / 32][32];
+#pragma unroll
+        for (int w = 0; w < kBK / 32; ++w) tmem_ld_32x32b_x32(s_addr + 32 * w, r[w]);
         tmem_ld_wait();
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          sv[e] = __uint_as_float(r0[e]);
-          sv[32 + e] = __uint_as_float(r1[e]);
-          sv[64 + e] = __uint_as_float(r2[e]);
-          sv[96 + e] = __uint_as_float(r3[e]);
-        }
+        for (int e = 0; e < kBK; ++e) sv[e] = __uint_as_float(r[e / 32][e % 32]);
       }
       const float smul = fmaxf(FP8 ? qmul * info->kmul : qmul, 1.17549435e-38f);  // not 0: -inf * 0
-      const int new_unit = info->unit;
+      const int new_unit = FP8 ? info->unit : 0;
       const int k0 = j * kBK;  // relative to lo
-      const uint32_t all4 = info->there[0] & info->there[1] & info->there[2] & info->there[3];
+      uint32_t all = info->there[0];
+#pragma unroll
+      for (int w = 1; w < kBK / 32; ++w) all &= info->there[w];
       // (a broken key is not in `there`: a tile may see all of a block that the span does not)
-      const bool need_mask = k0 < tile_lo || k0 + kBK > tile_hi || all4 != 0xffffffffu;
+      const bool need_mask = k0 < tile_lo || k0 + kBK > tile_hi || all != 0xffffffffu;
       if (need_mask) {
         uint32_t hit = 0;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+        for (int w = 0; w < kBK / 32; ++w) {
           // bits of keys k0 + 32 w + e in [see_lo, see_hi)
           const int f = min(max(see_lo - (k0 + 32 * w), 0), 32), e1 = min(max(see_hi - (k0 + 32 * w), 0), 32);
           uint32_t vis = info->there[w] | info->broken[w];
@@ -676,9 +649,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
         }
         broken_row |= hit != 0;
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&b->s_free[x]);
+      if constexpr (FP8) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&b->s_free[x]);
+      }
       float mxp[8];
 #pragma unroll
       for (int u = 0; u < 8; ++u) mxp[u] = fmaxf(sv[u], sv[8 + u]);
@@ -688,7 +663,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
         for (int u = 0; u < 8; ++u) mxp[u] = fmax3(mxp[u], sv[cc + u], sv[cc + 8 + u]);
       }
       const float mraw = fmax3(fmax3(mxp[0], mxp[1], mxp[2]), fmax3(mxp[3], mxp[4], mxp[5]), fmaxf(mxp[6], mxp[7]));
-      const float cand = mraw == -INFINITY ? -INFINITY : mraw * smul - kTopLog2;
+      const float cand = mraw == -INFINITY ? -INFINITY : mraw * smul - (FP8 ? kTopLog2 : 0.f);
       float alpha = 1.f;
       bool resc = cand > m_ref;
       if (resc) {
@@ -697,7 +672,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
       }
       const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
       const uint64_t negm2 = pk2(-m_use, -m_use), scale2 = pk2(smul, smul);
-      uint32_t pk[kBK / 2];
+      uint32_t pk[kBK / 2], pl[FP8 ? 1 : kBK / 2];  // bf16: pk is cut off after 8 bits, pl is the rest
       uint64_t rs2[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll
       for (int c8 = 0; c8 < kBK / 8; ++c8) {
@@ -708,7 +683,14 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
           x0 = ex2a(x0);
           x1 = ex2a(x1);
           rs2[e / 2] = add2(rs2[e / 2], pk2(x0, x1));
-          pk[c8 * 4 + e / 2] = h2_of(x0, x1);
+          if constexpr (FP8) {
+            pk[c8 * 4 + e / 2] = h2_of(x0, x1);
+          } else {
+            const uint32_t u0 = __float_as_uint(x0), u1 = __float_as_uint(x1);
+            pk[c8 * 4 + e / 2] = __byte_perm(u0, u1, 0x7632);
+            upk2(fma2(pk2(__uint_as_float(u0 & 0xffff0000u), __uint_as_float(u1 & 0xffff0000u)), pk2(-1.f, -1.f), pk2(x0, x1)), x0, x1);
+            pl[c8 * 4 + e / 2] = pack_bf16x2(x0, x1);
+          }
         }
       }
       float rs0, rs1;
@@ -736,14 +718,24 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
         }
       }
       {
-        uint32_t w0[32], w1[32];
+        uint32_t w0[32];
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          w0[e] = pk[e];
-          w1[e] = pk[32 + e];
-        }
+        for (int e = 0; e < 32; ++e) w0[e] = pk[e];
         tmem_st_32x32b_x32(p_addr, w0);
-        tmem_st_32x32b_x32(p_addr + 32, w1);
+        if constexpr (FP8) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) w0[e] = pk[32 + e];
+          tmem_st_32x32b_x32(p_addr + 32, w0);
+        } else {  // 48 columns of pk, then 48 of pl
+          uint32_t w1[32], w2[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            w1[e] = e < 16 ? pk[32 + e] : pl[e - 16];
+            w2[e] = pl[16 + e];
+          }
+          tmem_st_32x32b_x32(p_addr + 32, w1);
+          tmem_st_32x32b_x32(p_addr + 64, w2);
+        }
       }
       tmem_st_wait();
       tc_fence_before();
@@ -774,7 +766,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
     } else {
       inv = l_run == 0.f ? 0.f : 1.f / l_run;
     }
-    inv *= pow2i(max(unit, -127));
+    if constexpr (FP8) inv *= pow2i(max(unit, -127));
     bool bad = false;
 #pragma unroll
     for (int e = 0; e < 32; ++e) {
@@ -800,7 +792,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
     } else {
       // parts lie over the K/V tiles: [256 rows][64] fp32, 16-byte chunks swizzled by the row
       const int r = x * 128 + row;
-      const uint32_t dst = sbase + ChunkSmem::K + r * 256;
+      const uint32_t dst = sbase + C::K + r * 256;
 #pragma unroll
       for (int c16 = 0; c16 < 16; ++c16) {
         const uint32_t* s = c16 < 8 ? o0 + c16 * 4 : o1 + (c16 - 8) * 4;
@@ -810,7 +802,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
       b->row_l[r] = bad ? __uint_as_float(0x7fc00000u) : l_run;
       bad = false;
       cg::this_cluster().sync();
-      const float* part = reinterpret_cast<const float*>(smem + ChunkSmem::K);
+      const float* part = reinterpret_cast<const float*>(smem + C::K);
       for (int rr = rank * 8 + (warp - 4); rr < 256; rr += splits * 8) {
         const Tile& tt = rr < 128 ? tl[0] : tl[1];
         const int rt = (rr & 127) / a.group;
@@ -879,7 +871,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
 template <bool FP8>
 static void launch_chunk_t(const Args& a, int tokens, int slots, int splits, cudaStream_t stream) {
   auto kern = paged_chunk_kernel<FP8>;
-  constexpr int smem = ChunkSmem::INFO + 1024;
+  constexpr int smem = Cfg<FP8>::kBytes + 1024;
   static bool ready[64] = {};
   int dev;
   AF3_CUDA_CHECK(cudaGetDevice(&dev));

@@ -82,3 +82,13 @@ def test_large_value_without_weight(dev, q, ctx, hq, hkv, span):
         v[at] *= 2.0 ** span
     put(a, page, keys, k, v)
     check(a)
+
+
+@pytest.mark.parametrize("q,ctx", [(1, 700), (3, 300), (60, 500), (300, 1000), (64, 6000)])
+@pytest.mark.parametrize("power", [-20, -32, -60, 30])
+def test_channel_of_another_magnitude(dev, q, ctx, power):
+    """bf16 pages keep V's 8 bits at every magnitude, also in one channel among larger ones."""
+    a = make(dev, [q], [ctx], 16, 2, 16, False)
+    a["v_pages"][..., 5] *= 2.0 ** power
+    check(a)
+    check(a, window=100)
