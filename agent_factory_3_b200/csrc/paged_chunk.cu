@@ -429,7 +429,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
   } else if (warp < 4) {
     setmaxnreg_dec<72>();
     const int w = warp;
-    uint32_t top = 0;  // largest scale byte of V so far
+    uint32_t top = 0, low = 255;  // V's scale bytes so far: the largest, and the smallest that is not of zeros
     bool dead = false;
     Rows ah[kAhead];
     // Scale bytes of the block to expand.  Those of the next block are asked for at the top of a round
@@ -486,18 +486,18 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
       uint32_t kmax = __reduce_max_sync(0xffffffffu, kb), kmin = __reduce_min_sync(0xffffffffu, kb ? kb : 255u);
       if (lane == 0) b->red[n & 1][w] = vmax | (vmin << 8) | (kmax << 16) | (kmin << 24);
       named_barrier_sync(1, 128);
-      uint32_t most = 0, least = 255;
+      uint32_t most = 0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint32_t x = b->red[n & 1][i];
         most = max(most, x & 255u);
-        least = min(least, (x >> 8) & 255u);
+        low = min(low, (x >> 8) & 255u);
         kmax = max(kmax, (x >> 16) & 255u);
         kmin = min(kmin, x >> 24);
       }
       top = max(top, most);
       if (threadIdx.x == 0) {
-        if (least != 255u && (int)(top - least) > kWideRange) b->wide = 1;
+        if (low != 255u && (int)(top - low) > kWideRange) b->wide = 1;
         if (kmin != 255u && (int)(kmax - kmin) > kWideRange) b->wide = 1;
       }
       if (!dead && n >= kST && !mbar_wait(&b->kv_empty[st], ((n / kST) & 1) ^ 1, err, &b->abort_flag)) dead = true;

@@ -84,6 +84,27 @@ def test_large_value_without_weight(dev, q, ctx, hq, hkv, span):
     check(a)
 
 
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("span", [20, 45])
+@pytest.mark.parametrize("q,ctx", [(1, 300), (1, 3000), (3, 400), (60, 500), (200, 1000)])
+@pytest.mark.parametrize("first", [False, True])
+def test_large_value_of_little_weight(dev, q, ctx, span, first, fp8):
+    """A token of weight 2^-span of the largest and a value 2^span times the others' counts as much
+    as they do, whether it is met before them or after them."""
+    page, hq, hkv = 16, 8, 1
+    a = make(dev, [q], [ctx], hq, hkv, page, fp8)
+    a["sinks"] = torch.full((hq,), -20.0, device=dev)
+    u = torch.randn(64, device=dev).bfloat16()
+    a["q"] = u.repeat(q, hq).contiguous()
+    k = torch.zeros(ctx, hkv, 64, device=dev)
+    v = torch.randn(ctx, hkv, 64, device=dev)
+    at = 2 if first else ctx - q
+    k[at] = -8.0 * math.log(2.0 ** span) * u.float() / u.float().square().sum()
+    v[at] *= 2.0 ** span * ctx
+    put(a, page, torch.arange(ctx), k, v)
+    check(a)
+
+
 @pytest.mark.parametrize("q,ctx", [(1, 700), (3, 300), (60, 500), (300, 1000), (64, 6000)])
 @pytest.mark.parametrize("power", [-20, -32, -60, 30])
 def test_channel_of_another_magnitude(dev, q, ctx, power):
@@ -92,3 +113,20 @@ def test_channel_of_another_magnitude(dev, q, ctx, power):
     a["v_pages"][..., 5] *= 2.0 ** power
     check(a)
     check(a, window=100)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("q,ctx,window", [(1, 3000, 0), (5, 700, 0), (60, 500, 0), (60, 500, 400), (300, 1000, 0)])
+def test_large_values_in_all_later_blocks(dev, q, ctx, window, fp8):
+    """From key 384 on values are 2^45 times the earlier ones' at 2^-45 of their weight."""
+    page, hq, hkv = 16, 8, 1
+    a = make(dev, [q], [ctx], hq, hkv, page, fp8)
+    a["sinks"] = torch.full((hq,), -20.0, device=dev)
+    u = torch.randn(64, device=dev).bfloat16()
+    a["q"] = u.repeat(q, hq).contiguous()
+    k = torch.zeros(ctx, hkv, 64, device=dev)
+    v = torch.randn(ctx, hkv, 64, device=dev)
+    k[384:] = -8.0 * math.log(2.0 ** 45) * u.float() / u.float().square().sum()
+    v[384:] *= 2.0 ** 45
+    put(a, page, torch.arange(ctx), k, v)
+    check(a, window)
