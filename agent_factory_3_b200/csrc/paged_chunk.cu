@@ -131,6 +131,7 @@ __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
   asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
+constexpr uint32_t kNaN2 = 0x7e007e00u;  // f16 pair
 // f16 pair (2^e, 2^e) for e <= 0; 0 below f16's range
 __device__ __forceinline__ uint32_t h2_pow2(int e) {
   const uint32_t h = e >= -14 ? (uint32_t)(e + 15) << 10 : e >= -24 ? 1u << (e + 24) : 0u;
@@ -479,6 +480,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
 #pragma unroll
           for (int r = 0; r < 8; ++r) broken |= ((q >> (4 * r)) & 1u) << (8 * i + r);
         }
+        broken |= __ballot_sync(0xffffffffu, byte == 255u);
       }
       // ---- largest exponent of the block, and the smallest that is not of zeros
       const uint32_t vb = ((broken >> lane) & 1u) || byte == 255u ? 0u : byte, kb = kbyte == 255u ? 0u : kbyte;
@@ -504,7 +506,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
       // ---- expand into the f16 tile
       // (each key's lane works out its factor, and all of them travel before the first store: left
       // to the loop below, the stores kept the rows one after the other)
-      const uint32_t mine = h2_pow2(min((int)byte - (int)top, 0)), kmine = h2_pow2(min((int)kbyte - (int)kmax, 0));
+      // A scale byte of 255 (e8m0's NaN) makes the row NaN, or nothing where it is reported as broken.
+      const uint32_t mine = byte == 255u ? (partial ? 0u : kNaN2) : h2_pow2(min((int)byte - (int)top, 0));
       uint32_t mul[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) mul[i] = __shfl_sync(0xffffffffu, mine, 8 * i + (lane >> 2));
@@ -512,6 +515,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
       for (int i = 0; i < 4; ++i) expand16(vtile, 32 * w + 8 * i + (lane >> 2), lane & 3, v[i], mul[i]);
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[i] = lds4(own + (4 + i) * 2048);
+      const uint32_t kmine = kbyte == 255u ? kNaN2 : h2_pow2(min((int)kbyte - (int)kmax, 0));
 #pragma unroll
       for (int i = 0; i < 4; ++i) mul[i] = __shfl_sync(0xffffffffu, kmine, 8 * i + (lane >> 2));
 #pragma unroll

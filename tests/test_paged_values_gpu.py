@@ -64,6 +64,33 @@ def test_broken_value_that_whole_tiles_see(dev, fp8, q, start, hq, hkv, window, 
     assert torch.equal(torch.isnan(out.view(q, hq, 64)[..., 7]).all(1), sees)
 
 
+@pytest.mark.parametrize("q", [1, 3, 60, 300])
+@pytest.mark.parametrize("key", [5, 130, 399])
+def test_scale_byte_that_is_no_number(dev, q, key):
+    """A scale byte of 255 is no power of two (kv_store_fp8 never writes it): rows that see such a
+    value are not finite, the others are as they were."""
+    a = make(dev, [q], [400], 8, 1, 16, True)
+    want = check(a)
+    at = int(slots_of(a, 16)[key])
+    a["v_scales"][at // 16, :, at % 16] = 255
+    out = paged.paged_attention(**a, max_q_len=q, max_seq_len=400)
+    sees = 400 - q + torch.arange(q, device=dev) >= key
+    assert not torch.isfinite(out[sees]).any()
+    assert ((out[~sees] - want[~sees]).abs() <= 2.0 ** -7 * want[~sees].abs() + 1e-3).all()
+
+
+def test_scale_byte_that_is_no_number_in_k(dev):
+    """The same key by key, for few rows and in the kernel of long chunks."""
+    a = make(dev, [6], [400], 8, 1, 16, True)
+    at = int(slots_of(a, 16)[200])
+    a["k_scales"][at // 16, :, at % 16] = 255
+    few = paged.paged_attention(**a, max_q_len=5, max_seq_len=400)       # 40 rows
+    chunk = paged.paged_attention(**a, max_q_len=6, max_seq_len=400)     # 48 rows
+    assert torch.isnan(few).any() and torch.isfinite(few).any()      # scores of +inf and of -inf
+    assert torch.equal(torch.isnan(few), torch.isnan(chunk))
+    assert ((few - chunk).abs() <= 2.0 ** -7 * few.abs() + 1e-3)[torch.isfinite(few)].all()
+
+
 # ------------------------------------------------------------- magnitudes
 @pytest.mark.parametrize("span", [16, 28, 40, 60])
 @pytest.mark.parametrize("q,ctx,hq,hkv", [(1, 40, 16, 2), (1, 300, 8, 1), (1, 5000, 64, 8), (1, 700, 32, 1),
