@@ -41,7 +41,7 @@ __device__ __forceinline__ int exponent_of(uint32_t bits) {
 // One warp per row of qkv; its lanes walk the row's Hkv * D / 8 pieces of K and of V, 32 at a time.
 // The loads of both go out before anything waits, for the slot too.
 __global__ void __launch_bounds__(kCacheThreads) kv_store_fp8_kernel(const RowArgs a, const Pool p) {
-  const int row = (blockIdx.x * kCacheThreads + threadIdx.x) >> 5, lane = threadIdx.x & 31;
+  const int row = (int)blockIdx.x * (kCacheThreads / 32) + (int)(threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (row >= a.n) return;
   const uint32_t slot = (uint32_t)a.slots[row];
   const __nv_bfloat16* src = a.qkv + (int64_t)row * a.ld;
@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(kCacheThreads) kv_store_fp8_kernel(const RowAr
 
 // One warp per row of qkv, 64 pieces of K and of V at a time, every load before the first store.
 __global__ void __launch_bounds__(kCacheThreads) kv_gather_fp8_kernel(const RowArgs a, const Pool p) {
-  const int row = (blockIdx.x * kCacheThreads + threadIdx.x) >> 5, lane = threadIdx.x & 31;
+  const int row = (int)blockIdx.x * (kCacheThreads / 32) + (int)(threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (row >= a.n) return;
   const uint32_t slot = (uint32_t)a.slots[row];
   if (slot >= a.n_slots) return;
