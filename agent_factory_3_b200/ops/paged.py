@@ -79,6 +79,16 @@ def _slots(slots, k_pages):
     return ok, s // k_pages.shape[1], s % k_pages.shape[1]
 
 
+def _slots32(slots, k_pages):
+    """Slot ids as the kernels take them; ids of other types that are outside the pool become -1
+    before they are narrowed."""
+    if slots.dtype != torch.int32:
+        n = min(k_pages.shape[0] * k_pages.shape[1], 2 ** 31 - 1)
+        slots = slots.long()
+        slots = torch.where((slots >= 0) & (slots < n), slots, -1).to(torch.int32)
+    return slots if slots.is_contiguous() else slots.contiguous()
+
+
 def kv_store_fp8_reference(qkv, k_off, v_off, slots, k_pages, v_pages, k_scales, v_scales):
     _check_pages(k_pages, v_pages, k_scales, v_scales)
     _check(k_pages.dtype == FP8, "kv_store_fp8 needs float8_e4m3fn pages")
@@ -109,9 +119,7 @@ def kv_store_fp8(qkv, k_off, v_off, slots, k_pages, v_pages, k_scales, v_scales)
     pool (e.g. -1) is skipped; the others must be distinct."""
     if not use_cuda_kernels(qkv):
         return kv_store_fp8_reference(qkv, k_off, v_off, slots, k_pages, v_pages, k_scales, v_scales)
-    if slots.dtype != torch.int32 or not slots.is_contiguous():
-        slots = slots.to(torch.int32).contiguous()
-    ext().kv_store_fp8(qkv, k_off, v_off, slots, k_pages, v_pages, k_scales, v_scales)
+    ext().kv_store_fp8(qkv, k_off, v_off, _slots32(slots, k_pages), k_pages, v_pages, k_scales, v_scales)
 
 
 def kv_gather_fp8(qkv, k_off, v_off, slots, k_pages, v_pages, k_scales, v_scales) -> None:
@@ -119,9 +127,7 @@ def kv_gather_fp8(qkv, k_off, v_off, slots, k_pages, v_pages, k_scales, v_scales
     Rows of slots outside the pool keep what they hold."""
     if not use_cuda_kernels(qkv):
         return kv_gather_fp8_reference(qkv, k_off, v_off, slots, k_pages, v_pages, k_scales, v_scales)
-    if slots.dtype != torch.int32 or not slots.is_contiguous():
-        slots = slots.to(torch.int32).contiguous()
-    ext().kv_gather_fp8(qkv, k_off, v_off, slots, k_pages, v_pages, k_scales, v_scales)
+    ext().kv_gather_fp8(qkv, k_off, v_off, _slots32(slots, k_pages), k_pages, v_pages, k_scales, v_scales)
 
 
 def paged_attention_reference(q, k_pages, v_pages, page_table, seq_lens, cu_q, sinks, hq, hkv,

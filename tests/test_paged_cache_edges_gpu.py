@@ -1,4 +1,4 @@
-"""8-bit cache pages at the edges of their index types: very many rows."""
+"""8-bit cache pages at the edges of their index types: very many rows, slot ids in 64 bits."""
 import pytest
 import torch
 
@@ -9,6 +9,22 @@ def pool(device, pages=4, page=16, hkv=1, d=8):
     k, ks = paged.empty_fp8_pages(pages, page, hkv, d, device)
     v, vs = paged.empty_fp8_pages(pages, page, hkv, d, device)
     return k, v, ks, vs
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_slots_in_64_bits(device):
+    """A slot outside the pool is skipped, whatever its low 32 bits say."""
+    k, v, ks, vs = pool(device)
+    x = torch.arange(1, 7, device=device).float()[:, None].expand(6, 16).bfloat16().contiguous()
+    slots = torch.tensor([3, 2 ** 32 + 5, -2 ** 32 + 6, 64, -1, 7], device=device)
+    paged.kv_store_fp8(x, 0, 8, slots, k, v, ks, vs)
+    got = paged.dequantize_rows_reference(k.view(torch.uint8).view(paged.FP8), ks.transpose(1, 2))
+    want = torch.zeros(64, device=device)
+    want[3], want[7] = 1, 6
+    assert torch.equal(got.reshape(64, 8), want[:, None].expand(64, 8))
+    back = torch.full_like(x, 9.0)
+    paged.kv_gather_fp8(back, 0, 8, slots, k, v, ks, vs)
+    assert back[:, 0].tolist() == [1, 9, 9, 9, 9, 6]
 
 
 @pytest.mark.gpu
