@@ -199,7 +199,8 @@ def paged_attention(q, k_pages, v_pages, page_table, seq_lens, cu_q, sinks, hq, 
     p = seq_lens[b] - (cu_q[b+1] - cu_q[b]) + i and sees keys j <= p, with ``window`` only those
     with p - j < window.  A page id outside [0, pages) marks a page that is not held (any more):
     its keys are not visible.  ``sinks`` [Hq] joins the denominator (None: no sink).  A row that
-    sees nothing gets zeros; rows outside cu_q's ranges are not written.
+    sees nothing gets zeros; rows outside cu_q's ranges are not written.  There is no backward pass on
+    CUDA tensors: a q that asks for a gradient is refused.
 
     max_q_len / max_seq_len: the longest of each, if the caller knows them (otherwise they are
     read back from the device).  They choose the kernel variant and its split of the work; the
@@ -209,6 +210,8 @@ def paged_attention(q, k_pages, v_pages, page_table, seq_lens, cu_q, sinks, hq, 
         r = paged_attention_reference(q, k_pages, v_pages, page_table, seq_lens, cu_q, sinks, hq,
                                       hkv, window, scale, k_scales, v_scales).to(q.dtype)
         return r if out is None else out.copy_(r)
+    _check(not (q.requires_grad and torch.is_grad_enabled()),
+           "paged_attention has no backward pass: call it under torch.no_grad()")
     if q.dim() == 3:
         q = q.reshape(q.shape[0], -1)
     if scale is None:

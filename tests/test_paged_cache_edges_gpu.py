@@ -39,3 +39,17 @@ def test_more_than_2_27_rows():
     x.zero_()
     paged.kv_gather_fp8(x, 0, 0, slots, k, v, ks, vs)
     assert [float(x[i, 0]) for i in (0, 1, 2 ** 27, n - 1)] == [1.0, 0.0, 2.0, 3.0]
+
+
+@pytest.mark.gpu
+def test_no_silent_loss_of_a_gradient():
+    """The kernels have no backward pass: a q that asks for a gradient is refused."""
+    k, v = (torch.zeros(2, 16, 1, 64, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    args = (k, v, torch.zeros(1, 1, device="cuda", dtype=torch.int32),
+            torch.tensor([3], device="cuda", dtype=torch.int32),
+            torch.tensor([0, 1], device="cuda", dtype=torch.int32), None, 4, 1)
+    q = torch.randn(1, 256, device="cuda").bfloat16().requires_grad_()
+    with pytest.raises(RuntimeError, match="no backward"):
+        paged.paged_attention(q, *args)
+    with torch.no_grad():
+        assert (paged.paged_attention(q, *args) == 0).all()
