@@ -209,7 +209,12 @@ def paged_attention(q, k_pages, v_pages, page_table, seq_lens, cu_q, sinks, hq, 
     if not use_cuda_kernels(q):
         r = paged_attention_reference(q, k_pages, v_pages, page_table, seq_lens, cu_q, sinks, hq,
                                       hkv, window, scale, k_scales, v_scales).to(q.dtype)
-        return r if out is None else out.copy_(r)
+        if out is None:
+            return r
+        cu = cu_q.tolist()
+        for t0, t1 in zip(cu, cu[1:]):      # rows of no sequence are left as they are
+            out[t0:t1] = r[t0:t1]
+        return out
     _check(not (q.requires_grad and torch.is_grad_enabled()),
            "paged_attention has no backward pass: call it under torch.no_grad()")
     if q.dim() == 3:

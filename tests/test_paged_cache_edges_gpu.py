@@ -53,3 +53,15 @@ def test_no_silent_loss_of_a_gradient():
         paged.paged_attention(q, *args)
     with torch.no_grad():
         assert (paged.paged_attention(q, *args) == 0).all()
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_rows_of_no_sequence_are_not_written(device):
+    k, v = (torch.randn(2, 16, 1, 64, device=device).bfloat16() for _ in range(2))
+    q = torch.randn(6, 256, device=device).bfloat16()
+    out = torch.full((6, 256), 7.0, device=device, dtype=torch.bfloat16)
+    got = paged.paged_attention(q, k, v, torch.tensor([[0], [1]], device=device, dtype=torch.int32),
+                                torch.tensor([3, 9], device=device, dtype=torch.int32),
+                                torch.tensor([1, 2, 4], device=device, dtype=torch.int32), None, 4, 1,
+                                out=out)
+    assert got is out and (out[[0, 4, 5]] == 7).all() and (out[1:4] != 7).any(1).all()
