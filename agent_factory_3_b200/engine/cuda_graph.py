@@ -124,6 +124,8 @@ class DecodeGraphs:
         if not items or any(len(it.ids) != 1 or it.start <= 0 or it.all_logits or not it.want_logits
                             for it in items):
             return None
+        if self.runner.paged and not self.runner._pages_in_place():
+            return None
         B = _bucket(len(items))
         if B is None:
             return None

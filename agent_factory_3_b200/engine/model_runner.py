@@ -64,8 +64,8 @@ class ModelRunner:
         self.graphs = None      # engine.cuda_graph.DecodeGraphs when decode steps are captured
 
     def _pages_in_place(self) -> bool:
-        """Whether prefill chunks attend to the pages themselves: with ``paged``, where the head
-        dimension is the kernel's."""
+        """Whether steps attend to the pages themselves: with ``paged``, where the head dimension is
+        the kernel's.  With another one every item, decode rows too, gathers its context."""
         return self.paged and (self.cfg.head_dim == 64 or self.device.type != "cuda")
 
     def _qkv_lora(self, attn):
@@ -92,7 +92,8 @@ class ModelRunner:
             rows.append((r0, r0 + n))
             # a speculative verify block on top of cached pages is decoded row by row: its K/V
             # are stored first, so token j attends to start + j + 1 cached positions
-            decode = it.start > 0 and (n == 1 or (it.all_logits and not self.paged))
+            decode = it.start > 0 and (self._pages_in_place() and n == 1 if self.paged
+                                       else n == 1 or it.all_logits)
             (dec_idx if decode else pre_idx).append(i)
         m.N, m.rows, m.dec_idx, m.pre_idx = len(ids), rows, dec_idx, pre_idx
         m.ids_t = torch.tensor(ids, device=dev, dtype=torch.long)
@@ -201,10 +202,12 @@ class ModelRunner:
         elif m.pre_idx:
             ctx = torch.zeros(m.n_ctx, qkv.shape[1], device=dev, dtype=qkv.dtype)
             if ksc is not None:
+                # the new tokens' K and V too: as stored, like in every later step
                 P8.kv_gather_fp8(ctx, qs, qs + kvs, m.ctx_slots_t, kp, vp, ksc, vsc)
+                ctx[:, :qs].index_copy_(0, m.new_in_ctx_t, qkv[:, :qs].index_select(0, m.new_rows_t))
             else:
                 D.kv_gather(ctx, qs, qs + kvs, m.ctx_slots_t, kp, vp)
-            ctx.index_copy_(0, m.new_in_ctx_t, qkv.index_select(0, m.new_rows_t))
+                ctx.index_copy_(0, m.new_in_ctx_t, qkv.index_select(0, m.new_rows_t))
             if use_cuda_kernels(ctx) and d == 64:
                 oc = torch.empty(m.n_ctx, qs, device=dev, dtype=qkv.dtype)
                 lse = torch.empty(hq, m.n_ctx, device=dev, dtype=torch.float32)
