@@ -65,6 +65,22 @@ __device__ __forceinline__ float2 f16x2_to_float2(uint32_t h) {
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
+// Asynchronous copies of 16 bytes into shared memory, and its 16-byte loads.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
+  const int n = on ? 16 : 0;  // 0: the 16 bytes are filled with zeros and src is not read
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 r;
+  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(a));
+  return r;
+}
+
 // A byte, 0 where not on, in one predicated load: no branch for the result to be waited for in.
 __device__ __forceinline__ uint32_t load_byte(const uint8_t* p, bool on) {
   uint32_t r;

@@ -91,15 +91,6 @@ struct ChunkBars {
 };
 static_assert(sizeof(ChunkBars) <= 4096, "");
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool on) {
-  const int n = on ? 16 : 0;
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
-__device__ __forceinline__ uint4 lds4(uint32_t a) {
-  uint4 r;
-  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(a));
-  return r;
-}
 // 16-byte chunk c of row r of a 128B-swizzled tile of 128-byte rows
 __device__ __forceinline__ uint32_t sw128(int r, int c) { return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4)); }
 
@@ -265,12 +256,12 @@ __device__ __forceinline__ Rows load_rows(const Args& a, int page, int g, int ke
     const int64_t off = __shfl_sync(0xffffffffu, row, r) + c * 16;
     const bool there = (h.there >> r) & 1u;
     if constexpr (FP8) {
-      cp16(dst + i * 2048, a.p.v + off, there);
-      cp16(dst + (4 + i) * 2048, a.p.k + off, there);
+      cp_async16(dst + i * 2048, a.p.v + off, there);
+      cp_async16(dst + (4 + i) * 2048, a.p.k + off, there);
     } else {
       const uint32_t at = dst + sw128(r0 + r, c);
-      cp16(at, a.p.k + off, there);
-      cp16(at + (Cfg<false>::V - Cfg<false>::K), a.p.v + off, there);
+      cp_async16(at, a.p.k + off, there);
+      cp_async16(at + (Cfg<false>::V - Cfg<false>::K), a.p.v + off, there);
     }
   }
   return h;
@@ -294,7 +285,7 @@ __device__ __forceinline__ uint32_t clear_tile_rows(uint32_t tile, int r0) {
 #pragma unroll 1
   for (int i = 0; i < 8; ++i) {
     const uint32_t at = tile + sw128(r0 + 4 * i + (lane >> 3), lane & 7);
-    const uint4 w = lds4(at);
+    const uint4 w = lds128(at);
     uint32_t x[4] = {w.x, w.y, w.z, w.w}, bad = 0;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -402,12 +393,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
         there[i] = b0 + i < b1 ? load(b0 + i) : 0u;
-        asm volatile("cp.async.commit_group;" ::: "memory");
+        cp_async_commit();
       }
 #pragma unroll 1
       for (int j = b0; j < b1; ++j) {
         const int n = j - b0, st = n % kST, m = n + kAhead, k0 = lo + j * kBK;
-        asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
+        cp_async_wait<kAhead - 1>();
         uint32_t broken = 0;  // keys of this warp
         if (k0 < full_lo || k0 + kBK > full_hi) broken = clear_tile_rows(sbase + C::V + st * kTile, 32 * w);
         if (lane == 0) {
@@ -424,7 +415,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
           if (!dead && m >= kST && !mbar_wait(&b->kv_empty[m % kST], ((m / kST) & 1) ^ 1, err, &b->abort_flag)) dead = true;
           there[kAhead - 1] = load(j + kAhead);
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
+        cp_async_commit();
       }
     }
   } else if (warp < 4) {
@@ -449,7 +440,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
     for (int i = 0; i < kAhead; ++i) {
       ah[i] = Rows{0, 0};
       if (b0 + i < b1) ah[i] = load_rows<true>(a, pages[i], g, key0 + (b0 + i) * kBK, own0 + i * kTile, 0);
-      asm volatile("cp.async.commit_group;" ::: "memory");
+      cp_async_commit();
     }
     byte = fetch_scale(a.p.vs, ah[0]);
     kbyte = fetch_scale(a.p.ks, ah[0]);
@@ -458,13 +449,13 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
       const int n = j - b0, st = n % kST;
       const uint32_t next_byte = fetch_scale(a.p.vs, ah[1]), next_kbyte = fetch_scale(a.p.ks, ah[1]);
       const uint32_t own = own0 + raw_slot * kTile, vtile = sbase + C::V + st * kTile;
-      asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
+      cp_async_wait<kAhead - 1>();
       const int k0 = lo + j * kBK;
       const bool partial = k0 < full_lo || k0 + kBK > full_hi;
       uint32_t broken = 0;  // keys of this warp
       uint4 v[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = lds4(own + i * 2048);
+      for (int i = 0; i < 4; ++i) v[i] = lds128(own + i * 2048);
       if (partial) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -514,7 +505,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
 #pragma unroll
       for (int i = 0; i < 4; ++i) expand16(vtile, 32 * w + 8 * i + (lane >> 2), lane & 3, v[i], mul[i]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = lds4(own + (4 + i) * 2048);
+      for (int i = 0; i < 4; ++i) v[i] = lds128(own + (4 + i) * 2048);
       const uint32_t kmine = kbyte == 255u ? kNaN2 : h2_pow2(min((int)kbyte - (int)kmax, 0));
 #pragma unroll
       for (int i = 0; i < 4; ++i) mul[i] = __shfl_sync(0xffffffffu, kmine, 8 * i + (lane >> 2));
@@ -539,7 +530,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
         if (j + kAhead + 1 < b1) next_page = page_of(a, table, key0 + lane + (j + kAhead + 1) * kBK, hi);
         ah[kAhead - 1] = load_rows<true>(a, page, g, key0 + (j + kAhead) * kBK, own, 0);
       }
-      asm volatile("cp.async.commit_group;" ::: "memory");
+      cp_async_commit();
       byte = next_byte;
       kbyte = next_kbyte;
       raw_slot = raw_slot + 1 == kAhead ? 0 : raw_slot + 1;

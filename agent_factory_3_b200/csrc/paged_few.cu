@@ -67,22 +67,8 @@ struct FewCfg {
   static constexpr float kTop = FP8 ? 10.f : 0.f;  // the largest p of a row is 2^kTop
 };
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
-  const int n = on ? 16 : 0;  // 0: the 16 bytes are filled with zeros and src is not read
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-__device__ __forceinline__ uint4 lds128(uint32_t a) {
-  uint4 r;
-  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(a));
-  return r;
 }
 __device__ __forceinline__ uint2 lds64(uint32_t a) {
   uint2 r;
