@@ -86,7 +86,7 @@ def _slots32(slots, k_pages):
         n = min(k_pages.shape[0] * k_pages.shape[1], 2 ** 31 - 1)
         slots = slots.long()
         slots = torch.where((slots >= 0) & (slots < n), slots, -1).to(torch.int32)
-    return slots if slots.is_contiguous() else slots.contiguous()
+    return slots.contiguous()
 
 
 def kv_store_fp8_reference(qkv, k_off, v_off, slots, k_pages, v_pages, k_scales, v_scales):
@@ -119,7 +119,9 @@ def kv_store_fp8(qkv, k_off, v_off, slots, k_pages, v_pages, k_scales, v_scales)
     pool (e.g. -1) is skipped; the others must be distinct."""
     if not use_cuda_kernels(qkv):
         return kv_store_fp8_reference(qkv, k_off, v_off, slots, k_pages, v_pages, k_scales, v_scales)
-    ext().kv_store_fp8(qkv, k_off, v_off, _slots32(slots, k_pages), k_pages, v_pages, k_scales, v_scales)
+    if slots.dtype != torch.int32 or not slots.is_contiguous():
+        slots = _slots32(slots, k_pages)
+    ext().kv_store_fp8(qkv, k_off, v_off, slots, k_pages, v_pages, k_scales, v_scales)
 
 
 def kv_gather_fp8(qkv, k_off, v_off, slots, k_pages, v_pages, k_scales, v_scales) -> None:
@@ -127,7 +129,9 @@ def kv_gather_fp8(qkv, k_off, v_off, slots, k_pages, v_pages, k_scales, v_scales
     Rows of slots outside the pool keep what they hold."""
     if not use_cuda_kernels(qkv):
         return kv_gather_fp8_reference(qkv, k_off, v_off, slots, k_pages, v_pages, k_scales, v_scales)
-    ext().kv_gather_fp8(qkv, k_off, v_off, _slots32(slots, k_pages), k_pages, v_pages, k_scales, v_scales)
+    if slots.dtype != torch.int32 or not slots.is_contiguous():
+        slots = _slots32(slots, k_pages)
+    ext().kv_gather_fp8(qkv, k_off, v_off, slots, k_pages, v_pages, k_scales, v_scales)
 
 
 def paged_attention_reference(q, k_pages, v_pages, page_table, seq_lens, cu_q, sinks, hq, hkv,
@@ -215,8 +219,8 @@ def paged_attention(q, k_pages, v_pages, page_table, seq_lens, cu_q, sinks, hq, 
         for t0, t1 in zip(cu, cu[1:]):      # rows of no sequence are left as they are
             out[t0:t1] = r[t0:t1]
         return out
-    _check(not (q.requires_grad and torch.is_grad_enabled()),
-           "paged_attention has no backward pass: call it under torch.no_grad()")
+    if q.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("af3: paged_attention has no backward pass: call it under torch.no_grad()")
     if q.dim() == 3:
         q = q.reshape(q.shape[0], -1)
     if scale is None:
