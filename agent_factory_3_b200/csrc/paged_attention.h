@@ -8,11 +8,12 @@ namespace paged {
 constexpr int kFewRows = 32;  // query rows a KV head of launch_few's largest tile: its largest group
 
 // Sequences of up to this many query rows a KV head go to launch_few.  Measured on 4200 tokens, 8
-// heads a KV head, e4m3, launch_few against launch_chunk: 64 sequences of 4 tokens (32 rows) 198 and
-// 286 us, of 5 (40 rows) 259 and 253 us, of 8 (64 rows) 320 and 253 us; 8 sequences of 5: 44 and 58 us.
+// heads a KV head, 64 sequences, launch_few against launch_chunk: 4 tokens (32 rows) 197 and 285 us in
+// e4m3, 205 and 295 us in bf16; 5 (40 rows) 259 and 253 us, 303 and 262 us; ragged, 1 to 5 tokens on 210
+// to 4200, 115 and 220 us, 125 and 223 us.
 constexpr int kFewTotal = 40;
 
-// e4m3 pages: where the V (or K) scale bytes of keys that share a tile are further apart than this many
+// launch_few, e4m3 pages: where the V scale bytes of keys that share a tile are further apart than this many
 // powers of two, f16 no longer holds all of them well enough for a row in which the largest have little
 // weight or none; such a tile's rows are taken key by key.  At 14 the values at the small end still meet
 // weights of 2^-10 of the row's largest in 11 bits.  Tokens of one sequence differ by far less.

@@ -5,36 +5,35 @@
 // group) pair, floor(128 / group) tokens a tile, so the whole group shares every K/V block.  Few
 // spans over a long context are split: the CTAs of a cluster take parts of the keys and join over
 // distributed shared memory.
-//   warps 0-3    loaders, by cp.async (any page size and stride).  e4m3: 128-key blocks, three ahead,
-//                expanded into 128B-swizzled f16 tiles; bf16: 96-key blocks, four ahead, whose rows go
-//                straight into their tiles (three of the warps)
+//   warps 0-2    loaders of 96-key blocks by cp.async, four ahead (any page size and stride), 32 keys each:
+//                bf16 rows of K and V straight into 128B-swizzled tiles; e4m3 rows of V as raw pieces that
+//                the thread which copied them expands into a bf16 tile, scale included (code * 2^e is a
+//                bf16 number)
 //   warps 4-11   softmax, one warpgroup per 128-row tile: thread t owns query row t
-//   warp 12      tcgen05 issuer: S = Q K^T (M 128, N a block, K 64) of the next block is issued before
-//                O += P V (M 128, N 64, K a block, P from TMEM) of this one
-// Measured with 64 query heads on 8 KV heads: 4096 rows over 12288 cached keys 1.60 ms with e4m3 pages
-// (602 TFLOP/s), 1.75 ms with bf16.  The exponentials alone take 0.86 ms (16 a cycle and SM), the
-// softmax and the products without loaders 1.30 ms, loaders and products without softmax 0.85 ms
-// (e4m3).  The rest is the two getting in each other's way: issue slots of the softmax's dependent
-// instructions, and the instruction cache (3 to 7 % misses).  Tried and slower: K loaders of their own
-// for e4m3 (1.74 ms, 14 % misses), four softmax streams of 64 keys (1.83 ms), rolled loops in the
-// issuer (1.86 ms), spinning or sleeping waits.
+//   warp 12      tcgen05 issuer: S = Q K^T (M 128, N 96, K 64) of the next block is issued before
+//                O += P V (M 128, N 64, K 96, P from TMEM) of this one
+//   warps 13-15  e4m3: loaders of K, by the same instructions as V's
+// One bf16 P would cost as much precision as the rounding of the output, and an f16 P (11 bits down to
+// 2^-14, nothing below 2^-24) loses what a row gets from keys of little weight, which is all it has in a
+// channel where the others' codes are 0; V scaled to f16 has the like trouble with its own range.  So K, V and
+// Q are bf16 as they are, and P is two bf16 numbers, its first 8 bits and the next 8 (two products): nothing
+// depends on the magnitudes met elsewhere.  The softmax reference is the running maximum itself, so that a
+// row that one key dominates comes out as that key's value.
+// P takes as many TMEM columns as S and lies over it; two S of 96 columns a tile let the next block's
+// product start before this one's P is used (one S of 128: 2.04 ms where this takes 1.75).
+// TMEM: S / P of tile A 0 and 96, of tile B 192 and 288, O 384 and 448.
 //
-// One bf16 P would cost as much precision as the rounding of the output.
-//   bf16 pages: K, V and Q as they are; P as two bf16 numbers, its first 8 bits and the next 8 (two
-//               products), so that values of every magnitude keep their bits, next to any others.  P
-//               takes as many TMEM columns as S and lies over it; two S of 96 columns a tile let the
-//               next block's product start before this one's P is used (one S of 128: 2.04 ms).
-//               TMEM: S / P of tile A 0 and 96, of tile B 192 and 288, O 384 and 448.
-//   e4m3 pages: P as f16.  V' = code * 2^(e - u), with u the largest exponent the CTA has loaded (O is
-//               rescaled when u grows), K' = code * 2^(e - ek) with ek the block's largest exponent;
-//               both exact while a key's exponent is within kWideRange of the largest.
-//               TMEM: S 0 and 128, P 256 and 320, O 384 and 448.
-// The softmax reference is the running maximum itself: the largest p is 1 (bf16) or 2^10 (f16, which so
-// keeps 11 bits down to 2^-24 of it), and a row that one key dominates comes out as that key's value.
+// Measured with 64 query heads on 8 KV heads, 4096 rows over 12288 cached keys: bf16 pages 1.75 ms (550
+// TFLOP/s), e4m3 1.92 ms, where the loaders' expansion takes issue slots from the softmax's dependent
+// chains.  The exponentials alone take 0.86 ms (16 a cycle and SM).  e4m3 with f16 tiles and an f16 P took
+// 1.60 ms, but 30 of 600 random batches of widely spread scores were off by up to all of a small element
+// (of 32-bit torch's, 1).  Tried and slower for e4m3: one set of loaders for K and V (1.94 ms; a verify block
+// of 9 rows 210 against 196 us), two with instructions of their own (2.15 ms); for both: four softmax
+// streams of 64 keys, rolled loops in the issuer, spinning or sleeping waits.
 //
 // Rows that do not see a value must not meet it as 0 * inf: blocks that are not fully visible to
 // the whole span have such values cleared by the loaders and their keys reported; rows that do see
-// one, and e4m3 spans of too wide a range, are taken key by key at the end.
+// one are taken key by key at the end.
 #include <cooperative_groups.h>
 
 #include "common.h"
@@ -50,42 +49,36 @@ namespace paged {
 constexpr int kChunkThreads = 512;
 constexpr int kQTile = 128 * kD * 2;  // 16 KB: 128 rows of Q
 constexpr uint32_t kColO = 384;
-constexpr float kTopLog2 = 10.f;  // the largest p of a row is 2^10 (e4m3 pages; 1 for bf16)
+constexpr int kBK = 96;               // keys of a block
+constexpr int kLoaders = kBK / 32;    // warps, 32 keys each
+constexpr int kTile = kBK * kD * 2;   // 12 KB: a bf16 tile of K or V; e4m3: also a raw block
 
-// Blocks, stages and where things lie.
+// Stages and where things lie in shared memory.
 template <bool FP8>
 struct Cfg {
-  static constexpr int kBK = FP8 ? 128 : 96;     // keys of a block
-  static constexpr int kST = FP8 ? 4 : 6;        // stages of K/V tiles
-  static constexpr int kAhead = FP8 ? 3 : 4;     // blocks whose copies are in flight
-  static constexpr int kLoaders = kBK / 32;      // warps, 32 keys each
-  static constexpr int kTile = kBK * kD * 2;     // a 16-bit tile of K or V; e4m3: also a raw block
-  // shared memory
+  static constexpr int kST = FP8 ? 5 : 6;        // stages of K/V tiles
+  static constexpr int kAhead = 4;               // blocks whose copies are in flight
   static constexpr int Q = 0;                    // 2 tiles
   static constexpr int K = Q + 2 * kQTile;       // kST tiles
   static constexpr int V = K + kST * kTile;      // kST tiles
-  static constexpr int RAW = V + kST * kTile;    // e4m3: kAhead raw blocks, own 16-byte pieces of each loader thread
+  static constexpr int RAW = V + kST * kTile;    // e4m3: kAhead raw blocks, V's half and K's, own 16-byte pieces of each thread
   static constexpr int kBytes = RAW + (FP8 ? kAhead * kTile : 0);
-  static_assert(256 * kD * 4 <= kST * kTile, "a CTA's parts lie over its K tiles");
-  // TMEM columns of block c's S and P of tile x
-  __device__ static uint32_t col_s(int x, int c) { return FP8 ? x * 128 : x * 192 + (c & 1) * 96; }
-  __device__ static uint32_t col_p(int x, int c) { return FP8 ? 256 + x * 64 : col_s(x, c); }
+  static_assert(256 * kD * 4 <= 2 * kST * kTile, "a CTA's parts lie over its K and V tiles");
 };
+
+// TMEM column of block c's S, and of the P over it, of tile x
+__device__ __forceinline__ uint32_t col_s(int x, int c) { return x * 192 + (c & 1) * 96; }
 
 struct StageInfo {
   uint32_t there[4];   // keys that exist and lie in the span's range, but for the broken ones
   uint32_t broken[4];  // those whose V is not finite (cleared), in blocks not seen by every row
-  float kmul;          // e4m3: 2^ek
-  int unit;            // e4m3: V' is in units of 2^unit
 };
 
 constexpr int kMaxST = 6;
 struct ChunkBars {
-  uint64_t q_full, kv_full[kMaxST], kv_empty[kMaxST], s_full[2], s_free[2], p_full[2], o_ready[2];
+  uint64_t q_full, kv_full[kMaxST], kv_empty[kMaxST], s_full[2], p_full[2], o_ready[2];
   uint32_t tmem;
   int abort_flag;
-  int wide;
-  uint32_t red[2][4];
   StageInfo info[kMaxST];
   float row_m[256], row_l[256];
 };
@@ -112,20 +105,14 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-__device__ __forceinline__ uint32_t h2_of(float lo, float hi) {
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
   uint32_t r;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
-__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
-}
-constexpr uint32_t kNaN2 = 0x7e007e00u;  // f16 pair
-// f16 pair (2^e, 2^e) for e <= 0; 0 below f16's range
-__device__ __forceinline__ uint32_t h2_pow2(int e) {
-  const uint32_t h = e >= -14 ? (uint32_t)(e + 15) << 10 : e >= -24 ? 1u << (e + 24) : 0u;
+// bf16 pair of a scale byte's power of two, 2^(b - 127); 255: infinity
+__device__ __forceinline__ uint32_t scale_bf16x2(uint32_t b) {
+  const uint32_t h = b ? b << 7 : 0x40u;
   return h | (h << 16);
 }
 
@@ -135,7 +122,6 @@ struct Tile {
   int jlo, jhi;  // blocks, absolute; empty when jhi <= jlo
 };
 
-template <int kBK>
 __device__ __forceinline__ Tile make_tile(const Args& a, const Seq& s, int tok0, int tokens, int kv_lo, int b0, int b1) {
   Tile t;
   t.tok0 = tok0;
@@ -172,20 +158,15 @@ struct Issue {
   int jlo, jhi, n_s, n_pv;
 };
 
-template <bool FP8, int X>
+template <int X>
 __device__ __forceinline__ bool issue_s(Issue& t, int j, int st, uint32_t tmem, uint32_t sq, uint32_t sk0, ChunkBars* b,
                                         int* err) {
   if (j < t.jlo || j >= t.jhi) return true;
-  using C = Cfg<FP8>;
-  // e4m3: once S has been read; bf16: once the block before the last, whose P lies there, is done
-  if constexpr (FP8) {
-    if (t.n_s > 0 && !mbar_wait(&b->s_free[X], (t.n_s - 1) & 1, err, &b->abort_flag)) return false;
-  } else {
-    if (t.n_s > 1 && !mbar_wait(&b->o_ready[X], t.n_s & 1, err, &b->abort_flag)) return false;
-  }
+  // the block before the last, whose P lies there, has to be done
+  if (t.n_s > 1 && !mbar_wait(&b->o_ready[X], t.n_s & 1, err, &b->abort_flag)) return false;
   tc_fence_after();
-  constexpr uint32_t idesc = FP8 ? make_idesc_f16(128, C::kBK, false, false) : make_idesc_bf16(128, C::kBK, false, false);
-  const uint32_t q = sq + X * kQTile, k = sk0 + st * C::kTile, s = tmem + C::col_s(X, t.n_s);
+  constexpr uint32_t idesc = make_idesc_bf16(128, kBK, false, false);
+  const uint32_t q = sq + X * kQTile, k = sk0 + st * kTile, s = tmem + col_s(X, t.n_s);
 #pragma unroll
   for (int kk = 0; kk < kD / 16; ++kk)
     umma_f16(s, make_smem_desc(q + kk * 32, 16, 1024, kLayoutSW128),
@@ -195,20 +176,19 @@ __device__ __forceinline__ bool issue_s(Issue& t, int j, int st, uint32_t tmem, 
   return true;
 }
 
-template <bool FP8, int X>
+template <int X>
 __device__ __forceinline__ bool issue_pv(Issue& t, int j, int st, uint32_t tmem, uint32_t sv0, ChunkBars* b, int* err) {
   if (j < t.jlo || j >= t.jhi) return true;
-  using C = Cfg<FP8>;
   if (!mbar_wait(&b->p_full[X], t.n_pv & 1, err, &b->abort_flag)) return false;
   tc_fence_after();
-  constexpr uint32_t idesc = FP8 ? make_idesc_f16(128, kD, false, true) : make_idesc_bf16(128, kD, false, true);
-  const uint32_t v = sv0 + st * C::kTile, p = tmem + C::col_p(X, t.n_pv);
+  constexpr uint32_t idesc = make_idesc_bf16(128, kD, false, true);
+  const uint32_t v = sv0 + st * kTile, p = tmem + col_s(X, t.n_pv);
   const uint32_t first = t.n_pv > 0 ? 1u : 0u;
 #pragma unroll
-  for (int term = 0; term < (FP8 ? 1 : 2); ++term) {
+  for (int term = 0; term < 2; ++term) {
 #pragma unroll
-    for (int kk = 0; kk < C::kBK / 16; ++kk)
-      umma_f16_tmem_a(tmem + kColO + X * kD, p + term * (C::kBK / 2) + kk * 8,
+    for (int kk = 0; kk < kBK / 16; ++kk)
+      umma_f16_tmem_a(tmem + kColO + X * kD, p + term * (kBK / 2) + kk * 8,
                       make_smem_desc(v + kk * 2048, 8192, 1024, kLayoutSW128), idesc, term + kk > 0 ? 1u : first);
   }
   umma_commit(&b->o_ready[X]);
@@ -231,11 +211,12 @@ __device__ __forceinline__ int page_of(const Args& a, const int* table, int j, i
   return page;
 }
 
-// Starts the copies of keys key0 .. key0 + 31.  e4m3: 16 codes a piece, piece i of lane l is of row
-// 8 i + l / 4; V's go to own + i * 2048 (dst), K's after them.  bf16: 8 values a piece, of row
-// 4 i + l / 8, into rows r0 .. r0 + 31 of the swizzled tiles of K (dst) and V (as far behind).
+// Starts the copies of keys key0 .. key0 + 31.  e4m3: 16 codes a piece, piece i of lane l, of row
+// 8 i + l / 4 of `pool`, goes to dst + i * kPitch.  bf16: 8 values a piece, of row 4 i + l / 8 of both
+// pools, into rows r0 .. r0 + 31 of the swizzled tiles of K (dst) and V (as far behind).
+constexpr int kPitch = kLoaders * 32 * 16;  // of a loader thread's own pieces
 template <bool FP8>
-__device__ __forceinline__ Rows load_rows(const Args& a, int page, int g, int key0, uint32_t dst, int r0) {
+__device__ __forceinline__ Rows load_rows(const Args& a, const uint8_t* pool, int page, int g, int key0, uint32_t dst, int r0) {
   const int lane = threadIdx.x & 31;
   const bool on = (uint32_t)page < (uint32_t)a.p.num_pages;
   int64_t row = 0, sc = 0;
@@ -256,8 +237,7 @@ __device__ __forceinline__ Rows load_rows(const Args& a, int page, int g, int ke
     const int64_t off = __shfl_sync(0xffffffffu, row, r) + c * 16;
     const bool there = (h.there >> r) & 1u;
     if constexpr (FP8) {
-      cp_async16(dst + i * 2048, a.p.v + off, there);
-      cp_async16(dst + (4 + i) * 2048, a.p.k + off, there);
+      cp_async16(dst + i * kPitch, pool + off, there);
     } else {
       const uint32_t at = dst + sw128(r0 + r, c);
       cp_async16(at, a.p.k + off, there);
@@ -301,7 +281,7 @@ __device__ __forceinline__ uint32_t clear_tile_rows(uint32_t tile, int r0) {
   return broken;
 }
 
-// 16 e4m3 codes -> 16 f16 scaled by mul, into chunks 2c and 2c + 1 of row r.
+// 16 e4m3 codes -> 16 bf16 scaled by mul (exact), into chunks 2c and 2c + 1 of row r.
 __device__ __forceinline__ void expand16(uint32_t tile, int r, int c, const uint4& w, uint32_t mul) {
   const uint32_t x[4] = {w.x, w.y, w.z, w.w};
   uint32_t o[8];
@@ -309,8 +289,9 @@ __device__ __forceinline__ void expand16(uint32_t tile, int r, int c, const uint
   for (int i = 0; i < 4; ++i) {
     uint32_t l, h;
     e4m3x4_to_f16x2(x[i], l, h);
-    o[2 * i] = hmul2(l, mul);
-    o[2 * i + 1] = hmul2(h, mul);
+    const float2 fl = f16x2_to_float2(l), fh = f16x2_to_float2(h);
+    o[2 * i] = mul_bf16x2(pack_bf16x2(fl.x, fl.y), mul);
+    o[2 * i + 1] = mul_bf16x2(pack_bf16x2(fh.x, fh.y), mul);
   }
   st4(tile + sw128(r, 2 * c), o[0], o[1], o[2], o[3]);
   st4(tile + sw128(r, 2 * c + 1), o[4], o[5], o[6], o[7]);
@@ -320,7 +301,7 @@ template <bool FP8>
 __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Args a, const int tokens, const int splits,
                                                                       int* err) {
   using C = Cfg<FP8>;
-  constexpr int kBK = C::kBK, kST = C::kST, kAhead = C::kAhead, kTile = C::kTile;
+  constexpr int kST = C::kST, kAhead = C::kAhead;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ ChunkBars bars;
@@ -346,22 +327,20 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
   const int per = (nb + splits - 1) / splits;
   const int b0 = min(rank * per, nb), b1 = min(b0 + per, nb);
   const int* table = a.table + (int64_t)sb * a.ld_table;
-  const Tile tl[2] = {make_tile<kBK>(a, sq, tok0, tokens, lo, b0, b1), make_tile<kBK>(a, sq, tok0 + tokens, tokens, lo, b0, b1)};
+  const Tile tl[2] = {make_tile(a, sq, tok0, tokens, lo, b0, b1), make_tile(a, sq, tok0 + tokens, tokens, lo, b0, b1)};
 
   if (warp == 0 && lane == 0) {
     mbar_init(&b->q_full, 8);
     for (int s = 0; s < kST; ++s) {
-      mbar_init(&b->kv_full[s], C::kLoaders);
+      mbar_init(&b->kv_full[s], FP8 ? 2 * kLoaders : kLoaders);
       mbar_init(&b->kv_empty[s], 1);
     }
     for (int x = 0; x < 2; ++x) {
       mbar_init(&b->s_full[x], 1);
-      mbar_init(&b->s_free[x], 4);
       mbar_init(&b->p_full[x], 4);
       mbar_init(&b->o_ready[x], 1);
     }
     b->abort_flag = 0;
-    b->wide = 0;
     fence_barrier_init();
   }
   if (warp == 13) {
@@ -377,10 +356,29 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
   // a block is seen in full by every row of the span when it lies in [full_lo, full_hi)
   const int full_lo = a.window > 0 ? pos0 + ntok - a.window : 0, full_hi = min(pos0 + 1, sq.key_end);
 
-  // registers (launch: 512 x 128): loaders 72, softmax 2 x 184, issuer 72
+  auto issue = [&]() {
+    if (b1 > b0 && elect_one_sync()) {
+      const uint32_t sqa = sbase + C::Q, sk0 = sbase + C::K, sv0 = sbase + C::V;
+      Issue ta{tl[0].jlo, tl[0].jhi, 0, 0}, tb{tl[1].jlo, tl[1].jhi, 0, 0};
+      bool ok = mbar_wait(&b->q_full, 0, err, &b->abort_flag) && mbar_wait(&b->kv_full[0], 0, err, &b->abort_flag);
+      ok = ok && issue_s<0>(ta, b0, 0, tmem, sqa, sk0, b, err) && issue_s<1>(tb, b0, 0, tmem, sqa, sk0, b, err);
+      for (int j = b0; ok && j < b1; ++j) {
+        const int n = j - b0, st = n % kST, sn = (n + 1) % kST;
+        const bool next = j + 1 < b1;
+        if (next) ok = mbar_wait(&b->kv_full[sn], ((n + 1) / kST) & 1, err, &b->abort_flag);
+        if (ok && next) ok = issue_s<0>(ta, j + 1, sn, tmem, sqa, sk0, b, err);
+        ok = ok && issue_pv<0>(ta, j, st, tmem, sv0, b, err);
+        if (ok && next) ok = issue_s<1>(tb, j + 1, sn, tmem, sqa, sk0, b, err);
+        ok = ok && issue_pv<1>(tb, j, st, tmem, sv0, b, err);
+        umma_commit(&b->kv_empty[st]);
+      }
+    }
+  };
+
+  // registers (launch: 512 x 128): loaders and issuer 72, softmax 2 x 184
   if (!FP8 && warp < 4) {
     setmaxnreg_dec<72>();
-    if (warp < C::kLoaders) {
+    if (warp < kLoaders) {
       const int w = warp, key0 = lo + 32 * w;
       bool dead = false;
       uint32_t there[kAhead];
@@ -388,7 +386,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
       auto load = [&](int j) -> uint32_t {
         const int page = next_page;
         if (j + 1 < b1) next_page = page_of(a, table, key0 + lane + (j + 1) * kBK, hi);
-        return load_rows<false>(a, page, g, key0 + j * kBK, sbase + C::K + ((j - b0) % kST) * kTile, 32 * w).there;
+        return load_rows<false>(a, nullptr, page, g, key0 + j * kBK, sbase + C::K + ((j - b0) % kST) * kTile, 32 * w).there;
       };
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
@@ -418,141 +416,97 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
         cp_async_commit();
       }
     }
-  } else if (warp < 4) {
+  } else if (FP8 && (warp < 4 || warp >= 12)) {
     setmaxnreg_dec<72>();
-    const int w = warp;
-    uint32_t top = 0, low = 255;  // V's scale bytes so far: the largest, and the smallest that is not of zeros
-    bool dead = false;
-    Rows ah[kAhead];
-    // Scale bytes of the block to expand.  Those of the next block are asked for at the top of a round
-    // and moved here at its end: a move right after the load would wait for it (1000 cycles a block).
-    uint32_t byte = 0, kbyte = 0;
-    auto fetch_scale = [&](const uint8_t* from, const Rows& h) -> uint32_t {
-      return load_byte(from + h.scale, (h.there >> lane) & 1u);
-    };
-    const int key0 = lo + 32 * w;
-    int pages[kAhead];
+    if (warp < kLoaders || warp >= 13) {
+      const bool is_v = warp < 4;
+      const int w = is_v ? warp : warp - 13, key0 = lo + 32 * w;
+      const uint8_t *pool = is_v ? a.p.v : a.p.k, *scales = is_v ? a.p.vs : a.p.ks;
+      const uint32_t tile0 = sbase + (is_v ? C::V : C::K);
+      bool dead = false;
+      Rows ah[kAhead];
+      // Scale bytes of the block to expand.  Those of the next block are asked for at the top of a round
+      // and moved here at its end: a move right after the load would wait for it (1000 cycles a block).
+      uint32_t byte = 0;
+      auto fetch_scale = [&](const Rows& h) -> uint32_t {
+        return load_byte(scales + h.scale, (h.there >> lane) & 1u);
+      };
+      int pages[kAhead];
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) pages[i] = b0 + i < b1 ? page_of(a, table, key0 + lane + (b0 + i) * kBK, hi) : -1;
-    int next_page = b0 + kAhead < b1 ? page_of(a, table, key0 + lane + (b0 + kAhead) * kBK, hi) : -1;
-    const uint32_t own0 = sbase + C::RAW + (32 * w + lane) * 16;
+      for (int i = 0; i < kAhead; ++i) pages[i] = b0 + i < b1 ? page_of(a, table, key0 + lane + (b0 + i) * kBK, hi) : -1;
+      int next_page = b0 + kAhead < b1 ? page_of(a, table, key0 + lane + (b0 + kAhead) * kBK, hi) : -1;
+      const uint32_t own0 = sbase + C::RAW + (is_v ? 0 : 4 * kPitch) + (32 * w + lane) * 16;
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      ah[i] = Rows{0, 0};
-      if (b0 + i < b1) ah[i] = load_rows<true>(a, pages[i], g, key0 + (b0 + i) * kBK, own0 + i * kTile, 0);
-      cp_async_commit();
-    }
-    byte = fetch_scale(a.p.vs, ah[0]);
-    kbyte = fetch_scale(a.p.ks, ah[0]);
-    int raw_slot = 0;
-    for (int j = b0; j < b1; ++j) {
-      const int n = j - b0, st = n % kST;
-      const uint32_t next_byte = fetch_scale(a.p.vs, ah[1]), next_kbyte = fetch_scale(a.p.ks, ah[1]);
-      const uint32_t own = own0 + raw_slot * kTile, vtile = sbase + C::V + st * kTile;
-      cp_async_wait<kAhead - 1>();
-      const int k0 = lo + j * kBK;
-      const bool partial = k0 < full_lo || k0 + kBK > full_hi;
-      uint32_t broken = 0;  // keys of this warp
-      uint4 v[4];
+      for (int i = 0; i < kAhead; ++i) {
+        ah[i] = Rows{0, 0};
+        if (b0 + i < b1) ah[i] = load_rows<true>(a, pool, pages[i], g, key0 + (b0 + i) * kBK, own0 + i * kTile, 0);
+        cp_async_commit();
+      }
+      byte = fetch_scale(ah[0]);
+#pragma unroll 1
+      for (int j = b0; j < b1; ++j) {
+        const int n = j - b0, st = n % kST, k0 = lo + j * kBK;
+        const uint32_t next_byte = fetch_scale(ah[1]);
+        const uint32_t own = own0 + n % kAhead * kTile;
+        cp_async_wait<kAhead - 1>();
+        const bool partial = is_v && (k0 < full_lo || k0 + kBK > full_hi);
+        uint32_t broken = 0;  // keys of this warp
+        uint4 v[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = lds128(own + i * 2048);
-      if (partial) {
+        for (int i = 0; i < 4; ++i) v[i] = lds128(own + i * kPitch);
+        if (partial) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint32_t* x = reinterpret_cast<uint32_t*>(&v[i]);
-          bool bad = false;
+          for (int i = 0; i < 4; ++i) {
+            uint32_t* x = reinterpret_cast<uint32_t*>(&v[i]);
+            bool bad = false;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t m = __vcmpeq4(x[e] & 0x7f7f7f7fu, 0x7f7f7f7fu);
-            bad |= m != 0;
-            x[e] &= ~m;
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t m = __vcmpeq4(x[e] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+              bad |= m != 0;
+              x[e] &= ~m;
+            }
+            const uint32_t q = any_of_groups(__ballot_sync(0xffffffffu, bad), 4);  // bit 4 r: key 8 i + r
+#pragma unroll
+            for (int r = 0; r < 8; ++r) broken |= ((q >> (4 * r)) & 1u) << (8 * i + r);
           }
-          const uint32_t q = any_of_groups(__ballot_sync(0xffffffffu, bad), 4);  // bit 4 r: key 8 i + r
-#pragma unroll
-          for (int r = 0; r < 8; ++r) broken |= ((q >> (4 * r)) & 1u) << (8 * i + r);
+          broken |= __ballot_sync(0xffffffffu, byte == 255u);
         }
-        broken |= __ballot_sync(0xffffffffu, byte == 255u);
+        if (!dead && n >= kST && !mbar_wait(&b->kv_empty[st], ((n / kST) & 1) ^ 1, err, &b->abort_flag)) dead = true;
+        // ---- expand into the tiles
+        // (each key's lane works out its factor, and all of them travel before the first store: left
+        // to the loop below, the stores kept the rows one after the other)
+        const uint32_t mine = (broken >> lane) & 1u ? 0u : scale_bf16x2(byte);
+        uint32_t mul[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mul[i] = __shfl_sync(0xffffffffu, mine, 8 * i + (lane >> 2));
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          expand16(tile0 + st * kTile, 32 * w + 8 * i + (lane >> 2), lane & 3, v[i], mul[i]);
+        if (is_v && lane == 0) {
+          b->info[st].there[w] = ah[0].there & ~broken;
+          b->info[st].broken[w] = broken;
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&b->kv_full[st]);
+        // ---- refill
+#pragma unroll
+        for (int i = 0; i < kAhead - 1; ++i) ah[i] = ah[i + 1];
+        ah[kAhead - 1] = Rows{0, 0};
+        if (j + kAhead < b1) {
+          const int page = next_page;
+          if (j + kAhead + 1 < b1) next_page = page_of(a, table, key0 + lane + (j + kAhead + 1) * kBK, hi);
+          ah[kAhead - 1] = load_rows<true>(a, pool, page, g, key0 + (j + kAhead) * kBK, own, 0);
+        }
+        cp_async_commit();
+        byte = next_byte;
       }
-      // ---- largest exponent of the block, and the smallest that is not of zeros
-      const uint32_t vb = ((broken >> lane) & 1u) || byte == 255u ? 0u : byte, kb = kbyte == 255u ? 0u : kbyte;
-      const uint32_t vmax = __reduce_max_sync(0xffffffffu, vb), vmin = __reduce_min_sync(0xffffffffu, vb ? vb : 255u);
-      uint32_t kmax = __reduce_max_sync(0xffffffffu, kb), kmin = __reduce_min_sync(0xffffffffu, kb ? kb : 255u);
-      if (lane == 0) b->red[n & 1][w] = vmax | (vmin << 8) | (kmax << 16) | (kmin << 24);
-      named_barrier_sync(1, 128);
-      uint32_t most = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t x = b->red[n & 1][i];
-        most = max(most, x & 255u);
-        low = min(low, (x >> 8) & 255u);
-        kmax = max(kmax, (x >> 16) & 255u);
-        kmin = min(kmin, x >> 24);
-      }
-      top = max(top, most);
-      if (threadIdx.x == 0) {
-        if (low != 255u && (int)(top - low) > kWideRange) b->wide = 1;
-        if (kmin != 255u && (int)(kmax - kmin) > kWideRange) b->wide = 1;
-      }
-      if (!dead && n >= kST && !mbar_wait(&b->kv_empty[st], ((n / kST) & 1) ^ 1, err, &b->abort_flag)) dead = true;
-      // ---- expand into the f16 tile
-      // (each key's lane works out its factor, and all of them travel before the first store: left
-      // to the loop below, the stores kept the rows one after the other)
-      // A scale byte of 255 (e8m0's NaN) makes the row NaN, or nothing where it is reported as broken.
-      const uint32_t mine = byte == 255u ? (partial ? 0u : kNaN2) : h2_pow2(min((int)byte - (int)top, 0));
-      uint32_t mul[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) mul[i] = __shfl_sync(0xffffffffu, mine, 8 * i + (lane >> 2));
-#pragma unroll
-      for (int i = 0; i < 4; ++i) expand16(vtile, 32 * w + 8 * i + (lane >> 2), lane & 3, v[i], mul[i]);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = lds128(own + (4 + i) * 2048);
-      const uint32_t kmine = kbyte == 255u ? kNaN2 : h2_pow2(min((int)kbyte - (int)kmax, 0));
-#pragma unroll
-      for (int i = 0; i < 4; ++i) mul[i] = __shfl_sync(0xffffffffu, kmine, 8 * i + (lane >> 2));
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        expand16(sbase + C::K + st * kTile, 32 * w + 8 * i + (lane >> 2), lane & 3, v[i], mul[i]);
-      if (lane == 0) {
-        b->info[st].there[w] = ah[0].there & ~broken;
-        b->info[st].broken[w] = broken;
-      }
-      if (threadIdx.x == 0) b->info[st].kmul = pow2i((int)kmax - 127);
-      if (threadIdx.x == 0) b->info[st].unit = (int)top - 127;
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&b->kv_full[st]);
-      // ---- refill
-#pragma unroll
-      for (int i = 0; i < kAhead - 1; ++i) ah[i] = ah[i + 1];
-      ah[kAhead - 1] = Rows{0, 0};
-      if (j + kAhead < b1) {
-        const int page = next_page;
-        if (j + kAhead + 1 < b1) next_page = page_of(a, table, key0 + lane + (j + kAhead + 1) * kBK, hi);
-        ah[kAhead - 1] = load_rows<true>(a, page, g, key0 + (j + kAhead) * kBK, own, 0);
-      }
-      cp_async_commit();
-      byte = next_byte;
-      kbyte = next_kbyte;
-      raw_slot = raw_slot + 1 == kAhead ? 0 : raw_slot + 1;
+    } else if (warp == 12) {
+      issue();
     }
   } else if (warp >= 12) {
     setmaxnreg_dec<72>();
-    if (warp == 12 && b1 > b0 && elect_one_sync()) {
-      const uint32_t sqa = sbase + C::Q, sk0 = sbase + C::K, sv0 = sbase + C::V;
-      Issue ta{tl[0].jlo, tl[0].jhi, 0, 0}, tb{tl[1].jlo, tl[1].jhi, 0, 0};
-      bool ok = mbar_wait(&b->q_full, 0, err, &b->abort_flag) && mbar_wait(&b->kv_full[0], 0, err, &b->abort_flag);
-      ok = ok && issue_s<FP8, 0>(ta, b0, 0, tmem, sqa, sk0, b, err) && issue_s<FP8, 1>(tb, b0, 0, tmem, sqa, sk0, b, err);
-      for (int j = b0; ok && j < b1; ++j) {
-        const int n = j - b0, st = n % kST, sn = (n + 1) % kST;
-        const bool next = j + 1 < b1;
-        if (next) ok = mbar_wait(&b->kv_full[sn], ((n + 1) / kST) & 1, err, &b->abort_flag);
-        if (ok && next) ok = issue_s<FP8, 0>(ta, j + 1, sn, tmem, sqa, sk0, b, err);
-        ok = ok && issue_pv<FP8, 0>(ta, j, st, tmem, sv0, b, err);
-        if (ok && next) ok = issue_s<FP8, 1>(tb, j + 1, sn, tmem, sqa, sk0, b, err);
-        ok = ok && issue_pv<FP8, 1>(tb, j, st, tmem, sv0, b, err);
-        umma_commit(&b->kv_empty[st]);
-      }
-    }
+    if (warp == 12) issue();
   } else {
     setmaxnreg_inc<184>();
     const int x = (warp - 4) >> 2;
@@ -565,30 +519,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
     // visible keys of this row, relative to lo
     const int see_lo = a.window > 0 ? max(pos - a.window + 1, 0) - lo : -lo;
     const int see_hi = real ? min(pos + 1, sq.key_end) - lo : -1;  // exclusive
-    float qmul = a.scale_log2;
     {  // this row of Q into its tile
       const uint4* src = reinterpret_cast<const uint4*>(a.q + (int64_t)tok * a.ld_q + (int64_t)h * kD);
       const uint32_t dst = sbase + C::Q + x * kQTile;
       uint4 w[8];
 #pragma unroll
       for (int c = 0; c < 8; ++c) w[c] = real ? src[c] : make_uint4(0, 0, 0, 0);
-      if constexpr (FP8) {
-        uint32_t m2 = 0;
-#pragma unroll
-        for (int c = 0; c < 8; ++c)
-          m2 = __vmaxu2(m2, __vmaxu2(__vmaxu2(w[c].x & 0x7fff7fffu, w[c].y & 0x7fff7fffu),
-                                     __vmaxu2(w[c].z & 0x7fff7fffu, w[c].w & 0x7fff7fffu)));
-        int e = (int)(max(m2 & 0xffffu, m2 >> 16) >> 7) - 127;  // largest magnitude in [2^e, 2^(e+1))
-        if (e > 126 || e < -126) e = 0;
-        qmul *= pow2i(e);
-        const float f = pow2i(-e);
-#pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          uint32_t* q = reinterpret_cast<uint32_t*>(&w[c]);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) q[i] = h2_of(__uint_as_float(q[i] << 16) * f, __uint_as_float(q[i] & 0xffff0000u) * f);
-        }
-      }
 #pragma unroll
       for (int c = 0; c < 8; ++c) st4(dst + sw128(row, c), w[c].x, w[c].y, w[c].z, w[c].w);
       fence_proxy_async_smem();
@@ -600,8 +536,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
     // blocks [k0, k0 + 128) with every key visible to every row of the tile
     const int tile_lo = a.window > 0 ? max(t.pos0 + t.ntok - a.window, 0) - lo : -lo;
     const int tile_hi = min(t.pos0 + 1, sq.key_end) - lo;
+    const float smul = fmaxf(a.scale_log2, 1.17549435e-38f);  // not 0: -inf * 0
     float m_ref = -INFINITY, l_run = 0.f;
-    int unit = 0, c = 0;
+    int c = 0;
     bool ok = true, broken_row = false;
     for (int j = t.jlo; j < t.jhi; ++j, ++c) {
       const int st = (j - b0) % kST;
@@ -610,7 +547,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
           !mbar_wait(&b->kv_full[st], ((j - b0) / kST) & 1, err, &b->abort_flag)) { ok = false; break; }
       tc_fence_after();
       const StageInfo* info = &b->info[st];
-      const uint32_t s_addr = tmem + lane_base + C::col_s(x, c), p_addr = tmem + lane_base + C::col_p(x, c);
+      const uint32_t s_addr = tmem + lane_base + col_s(x, c);
       float sv[kBK];
       {
         uint32_t r[kBK / 32][32];
@@ -620,8 +557,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
 #pragma unroll
         for (int e = 0; e < kBK; ++e) sv[e] = __uint_as_float(r[e / 32][e % 32]);
       }
-      const float smul = fmaxf(FP8 ? qmul * info->kmul : qmul, 1.17549435e-38f);  // not 0: -inf * 0
-      const int new_unit = FP8 ? info->unit : 0;
       const int k0 = j * kBK;  // relative to lo
       uint32_t all = info->there[0];
 #pragma unroll
@@ -644,11 +579,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
         }
         broken_row |= hit != 0;
       }
-      if constexpr (FP8) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&b->s_free[x]);
-      }
       float mxp[8];
 #pragma unroll
       for (int u = 0; u < 8; ++u) mxp[u] = fmaxf(sv[u], sv[8 + u]);
@@ -658,7 +588,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
         for (int u = 0; u < 8; ++u) mxp[u] = fmax3(mxp[u], sv[cc + u], sv[cc + 8 + u]);
       }
       const float mraw = fmax3(fmax3(mxp[0], mxp[1], mxp[2]), fmax3(mxp[3], mxp[4], mxp[5]), fmaxf(mxp[6], mxp[7]));
-      const float cand = mraw == -INFINITY ? -INFINITY : mraw * smul - (FP8 ? kTopLog2 : 0.f);
+      const float cand = mraw == -INFINITY ? -INFINITY : mraw * smul;
       float alpha = 1.f;
       bool resc = cand > m_ref;
       if (resc) {
@@ -667,7 +597,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
       }
       const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
       const uint64_t negm2 = pk2(-m_use, -m_use), scale2 = pk2(smul, smul);
-      uint32_t pk[kBK / 2], pl[FP8 ? 1 : kBK / 2];  // bf16: pk is cut off after 8 bits, pl is the rest
+      uint32_t pk[kBK / 2], pl[kBK / 2];  // pk is cut off after 8 bits, pl is the rest
       uint64_t rs2[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll
       for (int c8 = 0; c8 < kBK / 8; ++c8) {
@@ -678,25 +608,15 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
           x0 = ex2a(x0);
           x1 = ex2a(x1);
           rs2[e / 2] = add2(rs2[e / 2], pk2(x0, x1));
-          if constexpr (FP8) {
-            pk[c8 * 4 + e / 2] = h2_of(x0, x1);
-          } else {
-            const uint32_t u0 = __float_as_uint(x0), u1 = __float_as_uint(x1);
-            pk[c8 * 4 + e / 2] = __byte_perm(u0, u1, 0x7632);
-            upk2(fma2(pk2(__uint_as_float(u0 & 0xffff0000u), __uint_as_float(u1 & 0xffff0000u)), pk2(-1.f, -1.f), pk2(x0, x1)), x0, x1);
-            pl[c8 * 4 + e / 2] = pack_bf16x2(x0, x1);
-          }
+          const uint32_t u0 = __float_as_uint(x0), u1 = __float_as_uint(x1);
+          pk[c8 * 4 + e / 2] = __byte_perm(u0, u1, 0x7632);
+          upk2(fma2(pk2(__uint_as_float(u0 & 0xffff0000u), __uint_as_float(u1 & 0xffff0000u)), pk2(-1.f, -1.f), pk2(x0, x1)), x0, x1);
+          pl[c8 * 4 + e / 2] = pack_bf16x2(x0, x1);
         }
       }
       float rs0, rs1;
       upk2(add2(add2(rs2[0], rs2[1]), add2(rs2[2], rs2[3])), rs0, rs1);
       l_run = l_run * alpha + (rs0 + rs1);
-      if (c == 0) unit = new_unit;
-      if (new_unit != unit) {
-        alpha *= pow2i(max(unit - new_unit, -127));
-        unit = new_unit;
-        resc = true;
-      }
       if (c > 0) {
         if (!mbar_wait(&b->o_ready[x], (c - 1) & 1, err, &b->abort_flag)) { ok = false; break; }
         tc_fence_after();
@@ -713,24 +633,16 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
         }
       }
       {
-        uint32_t w0[32];
+        uint32_t w0[32], w1[32], w2[32];  // 48 columns of pk, then 48 of pl
 #pragma unroll
-        for (int e = 0; e < 32; ++e) w0[e] = pk[e];
-        tmem_st_32x32b_x32(p_addr, w0);
-        if constexpr (FP8) {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) w0[e] = pk[32 + e];
-          tmem_st_32x32b_x32(p_addr + 32, w0);
-        } else {  // 48 columns of pk, then 48 of pl
-          uint32_t w1[32], w2[32];
-#pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            w1[e] = e < 16 ? pk[32 + e] : pl[e - 16];
-            w2[e] = pl[16 + e];
-          }
-          tmem_st_32x32b_x32(p_addr + 32, w1);
-          tmem_st_32x32b_x32(p_addr + 64, w2);
+        for (int e = 0; e < 32; ++e) {
+          w0[e] = pk[e];
+          w1[e] = e < 16 ? pk[32 + e] : pl[e - 16];
+          w2[e] = pl[16 + e];
         }
+        tmem_st_32x32b_x32(s_addr, w0);
+        tmem_st_32x32b_x32(s_addr + 32, w1);
+        tmem_st_32x32b_x32(s_addr + 64, w2);
       }
       tmem_st_wait();
       tc_fence_before();
@@ -748,8 +660,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
       tmem_ld_wait();
     }
     tc_fence_before();
-    named_barrier_sync(2, 256);  // every product of this CTA is done, b->wide is final
-    if (broken_row || b->wide) l_run = __uint_as_float(0x7fc00000u);  // NaN: key by key below
+    named_barrier_sync(2, 256);  // every product of this CTA is done
+    if (broken_row) l_run = __uint_as_float(0x7fc00000u);  // NaN: key by key below
     const float sk = a.sinks != nullptr ? a.sinks[h < a.hq ? h : 0] * kLog2e : -INFINITY;
     float inv, m_fin = m_ref;
     if (splits == 1) {
@@ -761,7 +673,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Arg
     } else {
       inv = l_run == 0.f ? 0.f : 1.f / l_run;
     }
-    if constexpr (FP8) inv *= pow2i(max(unit, -127));
     bool bad = false;
 #pragma unroll
     for (int e = 0; e < 32; ++e) {

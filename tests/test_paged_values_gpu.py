@@ -157,3 +157,22 @@ def test_large_values_in_all_later_blocks(dev, q, ctx, window, fp8):
     v[384:] *= 2.0 ** 45
     put(a, page, torch.arange(ctx), k, v)
     check(a, window)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("gap", [12, 18, 26, 60])
+@pytest.mark.parametrize("q,ctx", [(6, 200), (60, 500), (300, 400)])
+def test_channel_that_the_dominant_key_lacks(dev, q, ctx, gap, fp8):
+    """One key has all but e^-gap of a row's weight and zeros in some channels: there the row is what the
+    other keys give it."""
+    page, hq, hkv = 16, 8, 1
+    a = make(dev, [q], [ctx], hq, hkv, page, fp8)
+    a["sinks"] = None
+    u = torch.randn(64, device=dev).bfloat16()
+    a["q"] = u.repeat(q, hq).contiguous()
+    k = 0.05 * torch.randn(ctx, hkv, 64, device=dev)
+    k[7] = 8.0 * gap * u.float() / u.float().square().sum()
+    v = torch.randn(ctx, hkv, 64, device=dev)
+    v[7, :, ::5] = 0
+    put(a, page, torch.arange(ctx), k, v)
+    check(a)
