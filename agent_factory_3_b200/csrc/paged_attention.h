@@ -15,9 +15,9 @@ constexpr int kFewTotal = 40;
 
 // launch_few, e4m3 pages: where the V scale bytes of keys that share a tile are further apart than this many
 // powers of two, f16 no longer holds all of them well enough for a row in which the largest have little
-// weight or none; such a tile's rows are taken key by key.  At 14 the values at the small end still meet
-// weights of 2^-10 of the row's largest in 11 bits.  Tokens of one sequence differ by far less.
-constexpr int kWideRange = 14;
+// weight or none; such a tile's rows are taken key by key.  At 19 the values at the small end still meet
+// weights of 2^-10 of the row's largest (2^15) in 11 bits.  Tokens of one sequence differ by far less.
+constexpr int kWideRange = 19;
 
 // Few query rows a KV head and sequence, groups of at most kFewRows: memory-bound, split over the keys.
 void launch_few(const Args& a, int64_t max_q, int64_t max_len, cudaStream_t stream);

@@ -19,10 +19,11 @@
 //
 // e4m3 pages: codes are expanded to f16 (exact).  K's scale multiplies the score in fp32.  V's scale
 // is folded into P: P' = p * 2^(e - E) with E the largest V exponent seen by this warp so far; O is
-// rescaled when E grows.  The largest p is 2^10, so P' keeps f16's 11 bits down to 2^-24 of it; rows
-// that met exponents more than kWideRange apart are taken key by key (the values of the largest may
-// have next to no weight).  The query rows are brought to f16 after a power-of-two scaling to [1, 2),
-// undone in fp32.
+// rescaled when E grows.  The largest p is 2^15, so P' keeps f16's 11 bits down to 2^-29 of it (a key of
+// less weight counts with fewer bits, below 2^-39 not at all); rows that met exponents more than
+// kWideRange apart are taken key by key (the values of the largest may have next to no weight).  Codes
+// as bf16 and P' as two bf16 numbers would hold any range, at 18 % more time of the long decode (259 us).
+// The query rows are brought to f16 after a power-of-two scaling to [1, 2), undone in fp32.
 // (An e4m3 code costs one conversion of half rate; integer conversions took three times as long.)
 // bf16 pages: K, V, Q as they are; P as the sum of two bf16 numbers (16 bits), since one alone would
 // cost as much precision as the rounding of the output.  The 8 more instructions of 32 keys hide
@@ -64,7 +65,7 @@ struct FewCfg {
   static constexpr int kStageBytes = kSub * kSubBytes;
   static constexpr int kRingBytes = kStages * kStageBytes;
   static constexpr int kBlocksPerSm = LONG ? (kSub == 2 ? 3 : 1) : (NT == 1 ? 4 : NT == 2 ? 3 : 2);
-  static constexpr float kTop = FP8 ? 10.f : 0.f;  // the largest p of a row is 2^kTop
+  static constexpr float kTop = FP8 ? 15.f : 0.f;  // the largest p of a row is 2^kTop
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {

@@ -160,8 +160,10 @@ def test_large_values_in_all_later_blocks(dev, q, ctx, window, fp8):
 
 
 @pytest.mark.parametrize("fp8", [False, True])
-@pytest.mark.parametrize("gap", [12, 18, 26, 60])
-@pytest.mark.parametrize("q,ctx", [(6, 200), (60, 500), (300, 400)])
+@pytest.mark.parametrize("q,ctx,gap", [(q, ctx, gap) for q, ctx in ((6, 200), (60, 500), (300, 400))
+                                       for gap in (12, 18, 26, 60)]
+                         + [(q, ctx, gap) for q, ctx in ((1, 40), (1, 300), (1, 3000), (2, 2500), (3, 400))
+                            for gap in (12, 18)])      # few rows, e4m3: f16 holds 2^-29 of the largest weight
 def test_channel_that_the_dominant_key_lacks(dev, q, ctx, gap, fp8):
     """One key has all but e^-gap of a row's weight and zeros in some channels: there the row is what the
     other keys give it."""
