@@ -8,9 +8,9 @@ namespace paged {
 constexpr int kFewRows = 32;  // query rows a KV head of launch_few's largest tile: its largest group
 
 // Sequences of up to this many query rows a KV head go to launch_few.  Measured on 4200 tokens, 8
-// heads a KV head, 64 sequences, launch_few against launch_chunk: 4 tokens (32 rows) 197 and 285 us in
-// e4m3, 205 and 295 us in bf16; 5 (40 rows) 259 and 253 us, 303 and 262 us; ragged, 1 to 5 tokens on 210
-// to 4200, 115 and 220 us, 125 and 223 us.
+// heads a KV head, 64 sequences, launch_few against launch_chunk: 4 tokens (32 rows) 197 and 301 us in
+// e4m3, 205 and 295 us in bf16; 5 (40 rows) 259 and 279 us, 301 and 260 us; ragged, 1 to 5 tokens on 210
+// to 4200, 115 and 231 us, 125 and 223 us.
 constexpr int kFewTotal = 40;
 
 // launch_few, e4m3 pages: where the V scale bytes of keys that share a tile are further apart than this many

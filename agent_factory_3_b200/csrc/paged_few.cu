@@ -768,8 +768,8 @@ static void launch_few_nt(const Args& a, int rows_per_tile, int max_q, int64_t k
 template <bool FP8, bool LONG, bool ONE>
 static void launch_few_t(const Args& a, int max_q, int64_t keys, cudaStream_t stream) {
   // Up to 16 rows in one tile.  More rows take tiles of 16 that read the keys side by side, from L2
-  // but for one of them: 64 sequences of 5 tokens (40 rows) take 120 us so, 132 us in tiles of 32,
-  // whose registers leave half the warps.  A group of more than 16 heads needs the larger tile.
+  // but for one of them: 64 sequences of 5 tokens (40 rows) on 4200 take 259 us so, 341 us in tiles of
+  // 32, whose registers leave half the warps (e4m3; of 1 to 5 tokens on 210 to 4200, 115 and 133 us).  A group of more than 16 heads needs the larger tile.
   const int rows = a.group > 16 ? kFewRows : 16;
   const int want = std::max(std::min(max_q, rows / a.group), 1) * a.group;  // rows of a tile
   if (want <= 8)
