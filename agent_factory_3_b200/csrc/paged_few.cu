@@ -453,7 +453,7 @@ __global__ void __launch_bounds__(FewCfg<FP8, NT, LONG>::kThreads, FewCfg<FP8, N
           }
 #pragma unroll
           for (int u = 0; u < C::kSub; ++u) {
-            const float kf = __uint_as_float(info[s][u].k << 23);  // byte 0: below 2^-118, counts as 0
+            const float kf = __uint_as_float(max(info[s][u].k << 23, 0x400000u));  // (2^-127 is a denormal)
             const float vf = __uint_as_float((uint32_t)max(mine[u] - vmax + 127, 0) << 23);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {

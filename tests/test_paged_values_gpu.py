@@ -178,3 +178,17 @@ def test_channel_that_the_dominant_key_lacks(dev, q, ctx, gap, fp8):
     v[7, :, ::5] = 0
     put(a, page, torch.arange(ctx), k, v)
     check(a)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("q,ctx", [(1, 40), (1, 3000), (3, 400), (60, 500)])
+def test_keys_of_the_smallest_scale(dev, q, ctx, fp8):
+    """Keys of some 2^-121 (scale byte 0) meet queries of 2^120."""
+    page = 16
+    a = make(dev, [q], [ctx], 16, 2, page, fp8)
+    a["q"] = (torch.randn(q, 16 * 64, device=dev) * 2.0 ** 120).bfloat16()
+    put(a, page, torch.arange(ctx), torch.randn(ctx, 2, 64, device=dev) * 2.0 ** -121)
+    if fp8:
+        at = slots_of(a, page)
+        assert int(a["k_scales"][at // page, :, at % page].max()) == 0
+    check(a)
