@@ -8,7 +8,8 @@ once per layer for the whole batch.  Attention splits by kind:
     covers just the new rows).
 With ``paged`` (always so for a quantised cache) both kinds, and speculative verify blocks, attend
 to the pages in place instead (``ops.paged.paged_attention``): no context is gathered, and a verify
-block reads its context once rather than once per draft token.
+block reads its context once rather than once per draft token.  On CUDA that is for head dimension
+64; with another one every item of a ``paged`` runner gathers its context.
 New K/V go straight into their page slots; the MoE expert ids chosen for every new token are
 written next to them so routed experts can be returned for prefix-cache hits later.
 """
